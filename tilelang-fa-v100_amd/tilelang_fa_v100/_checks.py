@@ -50,7 +50,8 @@ def rows_ready(t: torch.Tensor) -> torch.Tensor:
             if size > 1 and (st % 8 != 0 or st < 0):
                 ok = False
                 break
-    return t if ok else t.contiguous()
+    # (clone: .contiguous() returns a contiguous tensor at an odd address as it is)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def strides(t: torch.Tensor, n: int) -> tuple:
