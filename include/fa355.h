@@ -326,6 +326,272 @@ typedef struct fa_cache_write_args {
 int fa_reshape_and_cache(const fa_cache_write_args* args, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Per-head RMS norm and position rotation of queries and keys.             */
+/*   q, k, q_out, k_out [batch, seqlen, heads, head_dim] (strides {batch,   */
+/*                seq, head}); in place (q_out == q with its strides) is    */
+/*                allowed                                                   */
+/*   q_weight, k_weight [head_dim] in fp32 (weight_f32) or dtype, or NULL:  */
+/*                no norm                                                   */
+/*   cos, sin     fp32 [num_positions, rotary_dim / 2] (row strides         */
+/*                table_stride[0] and [1])                                  */
+/*   positions    int64 (strides {batch, seq}), or NULL: the seq index      */
+/* x a head row, w its weight: n = x / sqrt(mean(x^2) + eps) * w in fp32;   */
+/* components i and i + rotary_dim / 2 (interleaved: 2 i and 2 i + 1) of n  */
+/* turn by table column i: (a cos - b sin, a sin + b cos); components from  */
+/* rotary_dim on stay.  One rounding, at the store.                         */
+/* A token with a negative position (padding) gets zero rows; one at or     */
+/* beyond num_positions gets NaN in its rotated components.                 */
+/* ------------------------------------------------------------------------ */
+typedef struct fa_norm_rope_args {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const void* q_weight;
+  const void* k_weight;
+  const float* cos;
+  const float* sin;
+  const int64_t* positions;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t qo_stride[3];
+  int64_t ko_stride[3];
+  int64_t table_stride[2]; /* multiples of 4 */
+  int64_t pos_stride[2];
+  int64_t num_positions;
+  int32_t batch;
+  int32_t seqlen;
+  int32_t num_heads;
+  int32_t num_heads_k;
+  int32_t head_dim;   /* multiple of 8 in [16, 512] */
+  int32_t rotary_dim; /* multiple of 16 in [16, head_dim] */
+  int32_t interleaved;
+  int32_t weight_f32;
+  int32_t dtype; /* fa_dtype of q, k, q_out, k_out */
+  float eps;
+} fa_norm_rope_args;
+
+/* No counterpart in the reference, whose callers rotate before they call it.
+ * No workspace. */
+int fa_norm_rope(const fa_norm_rope_args* args, void* stream);
+
+/* Backward of fa_norm_rope.  dq_out / dk_out: gradients of the outputs; dq /
+ * dk: of the inputs; dq_weight / dk_weight [head_dim], in the weights' type,
+ * NULL exactly where the weight is NULL (q / k are then not read and may be
+ * NULL).  Padding tokens have zero gradients.  The weights' gradients are
+ * summed in fp32 in a fixed order, through a workspace of
+ * fa_norm_rope_bwd_workspace_bytes (0 without weights) that depends on the
+ * current device's CU count. */
+typedef struct fa_norm_rope_bwd_args {
+  const void* q;
+  const void* k;
+  const void* dq_out;
+  const void* dk_out;
+  void* dq;
+  void* dk;
+  const void* q_weight;
+  const void* k_weight;
+  void* dq_weight;
+  void* dk_weight;
+  const float* cos;
+  const float* sin;
+  const int64_t* positions;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t dqo_stride[3];
+  int64_t dko_stride[3];
+  int64_t dq_stride[3];
+  int64_t dk_stride[3];
+  int64_t table_stride[2];
+  int64_t pos_stride[2];
+  int64_t num_positions;
+  int32_t batch;
+  int32_t seqlen;
+  int32_t num_heads;
+  int32_t num_heads_k;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t interleaved;
+  int32_t weight_f32;
+  int32_t dtype;
+  float eps;
+} fa_norm_rope_bwd_args;
+
+size_t fa_norm_rope_bwd_workspace_bytes(const fa_norm_rope_bwd_args* args);
+int fa_norm_rope_bwd(const fa_norm_rope_bwd_args* args, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* The serving form: fa_norm_rope on the new tokens' q and k, with k written
+ * to its slot of the paged cache and v copied to the same slot of the value
+ * cache (fa_reshape_and_cache's layout and slot rules: a slot outside the
+ * cache is skipped, its q row is still written).  Slots inside the cache must
+ * be distinct: a slot given twice ends with a mix of its tokens' components.
+ *   q, q_out [num_tokens, num_heads, head_dim], k, v [num_tokens,
+ *   num_kv_heads, head_dim] (strides {token, head}); positions int64
+ *   [num_tokens]; q_out must not overlap k or v. */
+typedef struct fa_norm_rope_cache_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  const int64_t* slot_mapping;
+  const int64_t* positions;
+  const void* q_weight;
+  const void* k_weight;
+  const float* cos;
+  const float* sin;
+  int64_t q_stride[2];
+  int64_t key_stride[2];
+  int64_t value_stride[2];
+  int64_t qo_stride[2];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t table_stride[2];
+  int64_t num_positions;
+  int32_t num_tokens;
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t page_size;
+  int32_t num_pages;
+  int32_t interleaved;
+  int32_t weight_f32;
+  int32_t dtype;
+  float eps;
+} fa_norm_rope_cache_args;
+
+/* No counterpart in the reference.  No workspace. */
+int fa_norm_rope_and_cache(const fa_norm_rope_cache_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Linear attention with a decay for each head.                             */
+/*   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T     (fp32, [head_dim (k),   */
+/*   o_t = scale q_t S_t                              head_dim (v)])         */
+/* log_decay fp32 [num_heads], natural log, <= 0 (-inf: no memory).         */
+/*   dense (query_start_loc NULL): q, out [batch, seqlen, num_heads,        */
+/*     head_dim], k, v [batch, seqlen, num_heads_k, head_dim] (strides      */
+/*     {batch, seq, head});                                                 */
+/*   packed: the same with one batch of num_tokens rows (the batch strides  */
+/*     are not read); sequence b is rows query_start_loc[b] ..              */
+/*     query_start_loc[b + 1] - 1, rows of no sequence stay as they were.   */
+/* Consecutive groups of num_heads / num_heads_k query heads share k and v. */
+/* States: initial_state / final_state fp32 with strides {slot, head}, each */
+/* [head_dim, head_dim] matrix contiguous; either may be NULL (zeros / not  */
+/* kept), and they may be the same memory.  Sequence b uses slot            */
+/* state_indices[b] (NULL: b); one outside [0, num_states) starts from zero */
+/* and keeps nothing; slots in use must be distinct.  prefix_kv_lens (NULL: */
+/* all start from the initial state): a sequence with prefix_kv_lens[b] <=  */
+/* 0 starts from zero.  A sequence of no tokens leaves its slot of          */
+/* final_state as it was.                                                   */
+/* The arithmetic: matrix products of dtype operands with fp32 sums; the    */
+/* states and every sum are fp32.                                           */
+/* ------------------------------------------------------------------------ */
+typedef struct fa_linear_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const float* log_decay;
+  const float* initial_state;
+  float* final_state;
+  const int32_t* query_start_loc; /* [batch + 1] or NULL */
+  const int32_t* prefix_kv_lens;  /* [batch] or NULL */
+  const int32_t* state_indices;   /* [batch] or NULL */
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t o_stride[3];
+  int64_t is_stride[2];
+  int64_t fs_stride[2];
+  int32_t batch;
+  int32_t seqlen; /* dense: tokens of a sequence; packed: all tokens (num_tokens) */
+  int32_t num_heads;
+  int32_t num_heads_k;
+  int32_t head_dim; /* 64, 128 or 256 */
+  int32_t num_states;
+  float scale;
+  int32_t dtype;
+} fa_linear_args;
+
+/* No counterpart in the reference.  The workspace (partial states of the
+ * sequences' segments; 0 bytes where there are none) depends on the sizes and
+ * the current device's CU count. */
+size_t fa_linear_fwd_workspace_bytes(const fa_linear_args* args);
+int fa_linear_fwd(const fa_linear_args* args, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
+/* Backward of the dense form.  dq / dk / dv as q / k / v; d_final_state
+ * (strides fs_stride, NULL: zeros) and d_initial_state (strides is_stride,
+ * NULL: not wanted) fp32.  No gradient for log_decay.  No atomics: gradients
+ * repeat bit for bit. */
+typedef struct fa_linear_bwd_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* dout;
+  void* dq;
+  void* dk;
+  void* dv;
+  const float* log_decay;
+  const float* initial_state;
+  const float* d_final_state;
+  float* d_initial_state;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t do_stride[3];
+  int64_t dq_stride[3];
+  int64_t dk_stride[3];
+  int64_t dv_stride[3];
+  int64_t is_stride[2];  /* initial_state */
+  int64_t fs_stride[2];  /* d_final_state */
+  int64_t dis_stride[2]; /* d_initial_state */
+  int32_t batch;
+  int32_t seqlen;
+  int32_t num_heads;
+  int32_t num_heads_k;
+  int32_t head_dim;
+  float scale;
+  int32_t dtype;
+} fa_linear_bwd_args;
+
+size_t fa_linear_bwd_workspace_bytes(const fa_linear_bwd_args* args);
+int fa_linear_bwd(const fa_linear_bwd_args* args, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
+/* One token for each sequence: state updated in place, then read.
+ *   q, out [batch, num_heads, head_dim], k, v [batch, num_heads_k, head_dim]
+ *   (strides {batch, head}); state fp32 (strides {slot, head}); state_indices
+ *   as above (a slot outside [0, num_states) starts from zero, keeps nothing).
+ * head_dim 64, 128 or 256.  fp32 arithmetic.  No workspace. */
+typedef struct fa_linear_decode_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const float* log_decay;
+  float* state;
+  const int32_t* state_indices;
+  int64_t q_stride[2];
+  int64_t k_stride[2];
+  int64_t v_stride[2];
+  int64_t o_stride[2];
+  int64_t s_stride[2];
+  int32_t batch;
+  int32_t num_heads;
+  int32_t num_heads_k;
+  int32_t head_dim;
+  int32_t num_states;
+  float scale;
+  int32_t dtype;
+} fa_linear_decode_args;
+
+int fa_linear_decode(const fa_linear_decode_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
 int fa_abi_version(void);
 const char* fa_strerror(int status);
 /* Message of the most recent failing call on this thread ("" if none). */

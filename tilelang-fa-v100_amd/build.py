@@ -25,8 +25,8 @@ BUILD = os.path.join(REPO, "_build")
 LIB = os.path.join(HERE, "tilelang_fa_v100", "libfa355.so")
 EXT = os.path.join(HERE, "tilelang_fa_v100", "_fa_torch.so")
 
-SOURCES = ["fa_fwd.hip", "fa_bwd.hip", "fa_decode.hip", "fa_cache.hip", "fa_scratch.hip",
-           "fa_capi.cpp"]
+SOURCES = ["fa_fwd.hip", "fa_bwd.hip", "fa_decode.hip", "fa_cache.hip", "fa_rope.hip",
+           "fa_linear.hip", "fa_scratch.hip", "fa_capi.cpp"]
 ARCH = "gfx950"
 
 # Per-source flags: MFMA results in VGPRs (the "VGPR form"; AGPRs then hold

@@ -12,6 +12,7 @@
 
 #include <cstdarg>
 #include <cstring>
+#include <initializer_list>
 
 #include "fa355.h"
 #include "fa_internal.h"
@@ -377,6 +378,252 @@ int fa_reshape_and_cache(const fa_cache_write_args* a, void* stream) {
   if (a->num_tokens == 0 || a->num_pages == 0) return ok();
   return hip_status(fa::launch_cache_write(*a, static_cast<hipStream_t>(stream)),
                     "fa_reshape_and_cache launch");
+}
+
+// ------------------------------------------------------------------ norm and rotation
+
+// What the three norm-and-rotation entry points share; tokens: rows of a head.
+extern "C++" {
+template <class Args>
+static int check_rope(const Args* a, const char* who, int64_t tokens, int heads_k) {
+  if (!a->cos || !a->sin) return fail(FA_E_INVALID, "%s: null table pointer", who);
+  if (a->dtype != FA_DTYPE_F16 && a->dtype != FA_DTYPE_BF16)
+    return fail(FA_E_UNSUPPORTED, "%s: dtype %d not supported", who, a->dtype);
+  if (a->head_dim < 16 || a->head_dim > 512 || (a->head_dim & 7) != 0)
+    return fail(FA_E_UNSUPPORTED, "%s: head_dim %d not a multiple of 8 in [16, 512]", who,
+                a->head_dim);
+  if (a->rotary_dim < 16 || a->rotary_dim > a->head_dim || (a->rotary_dim & 15) != 0)
+    return fail(FA_E_UNSUPPORTED, "%s: rotary_dim %d not a multiple of 16 in [16, head_dim]", who,
+                a->rotary_dim);
+  if (tokens < 0 || a->num_heads <= 0 || heads_k <= 0 || a->num_positions <= 0)
+    return fail(FA_E_INVALID, "%s: bad size", who);
+  if (!aligned16(a->cos) || !aligned16(a->sin) || a->table_stride[0] < 0 ||
+      a->table_stride[1] < 0 || (a->table_stride[0] & 3) != 0 || (a->table_stride[1] & 3) != 0)
+    return fail(FA_E_UNSUPPORTED,
+                "%s: cos / sin must be 16-byte aligned with row strides that are multiples of 4",
+                who);
+  if (!aligned16(a->q_weight) || !aligned16(a->k_weight))
+    return fail(FA_E_UNSUPPORTED, "%s: weights must be 16-byte aligned", who);
+  // Rows are counted in 31 bits on the device.
+  if (tokens > kIntMax / (a->num_heads > heads_k ? a->num_heads : heads_k))
+    return fail(FA_E_UNSUPPORTED, "%s: problem too large", who);
+  return ok();
+}
+}
+
+static int check_rows(const char* who, std::initializer_list<const void*> ptrs,
+                      std::initializer_list<const int64_t*> strides, int n) {
+  for (const void* p : ptrs) {
+    if (!p) return fail(FA_E_INVALID, "%s: null tensor pointer", who);
+    if (!aligned16(p)) return fail(FA_E_UNSUPPORTED, "%s: tensors must be 16-byte aligned", who);
+  }
+  for (const int64_t* s : strides)
+    if (!strides_ok(s, n))
+      return fail(FA_E_UNSUPPORTED, "%s: strides must be non-negative multiples of 8", who);
+  return ok();
+}
+
+static bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+static bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+int fa_norm_rope(const fa_norm_rope_args* a, void* stream) {
+  const char* who = "fa_norm_rope";
+  if (!a) return fail(FA_E_INVALID, "%s: null args", who);
+  if (a->batch < 0 || a->seqlen < 0) return fail(FA_E_INVALID, "%s: negative size", who);
+  const int64_t tokens = (int64_t)a->batch * a->seqlen;
+  int st = check_rope(a, who, tokens, a->num_heads_k);
+  if (st != FA_OK) return st;
+  st = check_rows(who, {a->q, a->k, a->q_out, a->k_out},
+                  {a->q_stride, a->k_stride, a->qo_stride, a->ko_stride}, 3);
+  if (st != FA_OK) return st;
+  if (!aligned8(a->positions))
+    return fail(FA_E_INVALID, "%s: positions must be 8-byte aligned", who);
+  if (tokens == 0) return ok();
+  return hip_status(fa::launch_norm_rope(*a, static_cast<hipStream_t>(stream)),
+                    "fa_norm_rope launch");
+}
+
+static int check_rope_bwd(const fa_norm_rope_bwd_args* a) {
+  const char* who = "fa_norm_rope_bwd";
+  if (!a) return fail(FA_E_INVALID, "%s: null args", who);
+  if (a->batch < 0 || a->seqlen < 0) return fail(FA_E_INVALID, "%s: negative size", who);
+  int st = check_rope(a, who, (int64_t)a->batch * a->seqlen, a->num_heads_k);
+  if (st != FA_OK) return st;
+  st = check_rows(who, {a->dq_out, a->dk_out, a->dq, a->dk},
+                  {a->dqo_stride, a->dko_stride, a->dq_stride, a->dk_stride}, 3);
+  if (st != FA_OK) return st;
+  if (a->q_weight && (st = check_rows(who, {a->q}, {a->q_stride}, 3)) != FA_OK) return st;
+  if (a->k_weight && (st = check_rows(who, {a->k}, {a->k_stride}, 3)) != FA_OK) return st;
+  if (!a->q_weight != !a->dq_weight || !a->k_weight != !a->dk_weight)
+    return fail(FA_E_INVALID, "%s: a weight and its gradient go together", who);
+  if (!aligned4(a->dq_weight) || !aligned4(a->dk_weight))
+    return fail(FA_E_UNSUPPORTED, "%s: weight gradients must be 4-byte aligned", who);
+  if (!aligned8(a->positions))
+    return fail(FA_E_INVALID, "%s: positions must be 8-byte aligned", who);
+  return ok();
+}
+
+size_t fa_norm_rope_bwd_workspace_bytes(const fa_norm_rope_bwd_args* a) {
+  if (check_rope_bwd(a) != FA_OK) return 0;
+  return fa::norm_rope_bwd_workspace_bytes(*a);
+}
+
+int fa_norm_rope_bwd(const fa_norm_rope_bwd_args* a, void* ws, size_t ws_bytes, void* stream) {
+  const int st = check_rope_bwd(a);
+  if (st != FA_OK) return st;
+  const size_t need = fa::norm_rope_bwd_workspace_bytes(*a);
+  if (need > 0 && (!ws || ws_bytes < need || !aligned16(ws)))
+    return fail(FA_E_WORKSPACE,
+                "fa_norm_rope_bwd: workspace needs %zu bytes (16-byte aligned), got %zu", need,
+                ws ? ws_bytes : (size_t)0);
+  return hip_status(fa::launch_norm_rope_bwd(*a, ws, static_cast<hipStream_t>(stream)),
+                    "fa_norm_rope_bwd launch");
+}
+
+int fa_norm_rope_and_cache(const fa_norm_rope_cache_args* a, void* stream) {
+  const char* who = "fa_norm_rope_and_cache";
+  if (!a) return fail(FA_E_INVALID, "%s: null args", who);
+  int st = check_rope(a, who, a->num_tokens, a->num_kv_heads);
+  if (st != FA_OK) return st;
+  st = check_rows(who, {a->q, a->k, a->v, a->q_out},
+                  {a->q_stride, a->key_stride, a->value_stride, a->qo_stride}, 2);
+  if (st != FA_OK) return st;
+  st = check_rows(who, {a->k_cache, a->v_cache}, {a->k_stride, a->v_stride}, 3);
+  if (st != FA_OK) return st;
+  if (!a->slot_mapping || !a->positions) return fail(FA_E_INVALID, "%s: null pointer", who);
+  if (!aligned8(a->slot_mapping) || !aligned8(a->positions))
+    return fail(FA_E_INVALID, "%s: slot_mapping and positions must be 8-byte aligned", who);
+  if (a->page_size <= 0 || a->num_pages < 0) return fail(FA_E_INVALID, "%s: bad size", who);
+  if (a->num_tokens == 0) return ok();
+  return hip_status(fa::launch_norm_rope_cache(*a, static_cast<hipStream_t>(stream)),
+                    "fa_norm_rope_and_cache launch");
+}
+
+// ------------------------------------------------------------------ linear attention
+
+extern "C++" {
+template <class Args>
+static int check_linear(const Args* a, const char* who) {
+  if (!a->log_decay) return fail(FA_E_INVALID, "%s: null log_decay", who);
+  if (a->dtype != FA_DTYPE_F16 && a->dtype != FA_DTYPE_BF16)
+    return fail(FA_E_UNSUPPORTED, "%s: dtype %d not supported", who, a->dtype);
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256)
+    return fail(FA_E_UNSUPPORTED, "%s: head_dim %d not in {64,128,256}", who, a->head_dim);
+  if (a->batch < 0) return fail(FA_E_INVALID, "%s: negative size", who);
+  if (a->num_heads <= 0 || a->num_heads_k <= 0 || a->num_heads % a->num_heads_k != 0)
+    return fail(FA_E_INVALID, "%s: num_heads %d not a multiple of num_heads_k %d", who,
+                a->num_heads, a->num_heads_k);
+  return ok();
+}
+}
+
+// A state array of fp32 matrices that the kernels address in 16-byte pieces.
+static int check_state(const char* who, const float* s, const int64_t (&stride)[2]) {
+  if (!s) return ok();
+  if (!aligned16(s) || stride[0] < 0 || stride[1] < 0 || (stride[0] & 3) != 0 ||
+      (stride[1] & 3) != 0)
+    return fail(FA_E_UNSUPPORTED,
+                "%s: states must be 16-byte aligned with strides that are multiples of 4", who);
+  return ok();
+}
+
+// Workgroups of one launch: sequences x heads x up to 64 parts of a state, and
+// the segments.
+static int check_linear_grid(const char* who, int64_t batch, int heads, int D, int64_t groups) {
+  if (batch * heads > kIntMax / (D * D / 1024) || groups > kIntMax)
+    return fail(FA_E_UNSUPPORTED, "%s: problem too large", who);
+  return ok();
+}
+
+static int check_linear_fwd(const fa_linear_args* a) {
+  const char* who = "fa_linear_fwd";
+  if (!a) return fail(FA_E_INVALID, "%s: null args", who);
+  int st = check_linear(a, who);
+  if (st != FA_OK) return st;
+  if (a->seqlen < 0 || a->num_states < 0) return fail(FA_E_INVALID, "%s: negative size", who);
+  st = check_rows(who, {a->q, a->k, a->v, a->out},
+                  {a->q_stride, a->k_stride, a->v_stride, a->o_stride}, 3);
+  if (st != FA_OK) return st;
+  if ((st = check_state(who, a->initial_state, a->is_stride)) != FA_OK) return st;
+  if ((st = check_state(who, a->final_state, a->fs_stride)) != FA_OK) return st;
+  // The rows of a sequence are counted in int, rounded up to whole segments.
+  if (a->seqlen > kIntMax / 2) return fail(FA_E_UNSUPPORTED, "%s: problem too large", who);
+  return check_linear_grid(who, a->batch, a->num_heads, a->head_dim,
+                           a->batch && a->seqlen ? fa::linear_fwd_workgroups(*a) : 0);
+}
+
+size_t fa_linear_fwd_workspace_bytes(const fa_linear_args* a) {
+  if (check_linear_fwd(a) != FA_OK || a->batch == 0 || a->seqlen == 0) return 0;
+  return fa::linear_fwd_workspace_bytes(*a);
+}
+
+int fa_linear_fwd(const fa_linear_args* a, void* ws, size_t ws_bytes, void* stream) {
+  const int st = check_linear_fwd(a);
+  if (st != FA_OK) return st;
+  if (a->batch == 0 || a->seqlen == 0) return ok();
+  const size_t need = fa::linear_fwd_workspace_bytes(*a);
+  if (need > 0 && (!ws || ws_bytes < need || !aligned16(ws)))
+    return fail(FA_E_WORKSPACE,
+                "fa_linear_fwd: workspace needs %zu bytes (16-byte aligned), got %zu", need,
+                ws ? ws_bytes : (size_t)0);
+  return hip_status(fa::launch_linear_fwd(*a, ws, static_cast<hipStream_t>(stream)),
+                    "fa_linear_fwd launch");
+}
+
+static int check_linear_bwd(const fa_linear_bwd_args* a) {
+  const char* who = "fa_linear_bwd";
+  if (!a) return fail(FA_E_INVALID, "%s: null args", who);
+  int st = check_linear(a, who);
+  if (st != FA_OK) return st;
+  if (a->seqlen < 0) return fail(FA_E_INVALID, "%s: negative size", who);
+  st = check_rows(who, {a->q, a->k, a->v, a->dout, a->dq, a->dk, a->dv},
+                  {a->q_stride, a->k_stride, a->v_stride, a->do_stride, a->dq_stride,
+                   a->dk_stride, a->dv_stride}, 3);
+  if (st != FA_OK) return st;
+  if ((st = check_state(who, a->initial_state, a->is_stride)) != FA_OK) return st;
+  if ((st = check_state(who, a->d_final_state, a->fs_stride)) != FA_OK) return st;
+  if ((st = check_state(who, a->d_initial_state, a->dis_stride)) != FA_OK) return st;
+  if (a->seqlen > kIntMax / 2 ||
+      (int64_t)a->batch * a->seqlen > (int64_t)kIntMax * 4 / a->num_heads_k)
+    return fail(FA_E_UNSUPPORTED, "%s: problem too large", who);
+  return check_linear_grid(who, a->batch, a->num_heads, a->head_dim,
+                           a->batch && a->seqlen ? fa::linear_bwd_workgroups(*a) : 0);
+}
+
+size_t fa_linear_bwd_workspace_bytes(const fa_linear_bwd_args* a) {
+  if (check_linear_bwd(a) != FA_OK || a->batch == 0 || a->seqlen == 0) return 0;
+  return fa::linear_bwd_workspace_bytes(*a);
+}
+
+int fa_linear_bwd(const fa_linear_bwd_args* a, void* ws, size_t ws_bytes, void* stream) {
+  const int st = check_linear_bwd(a);
+  if (st != FA_OK) return st;
+  if (a->batch == 0 || a->seqlen == 0) return ok();
+  const size_t need = fa::linear_bwd_workspace_bytes(*a);
+  if (need > 0 && (!ws || ws_bytes < need || !aligned16(ws)))
+    return fail(FA_E_WORKSPACE,
+                "fa_linear_bwd: workspace needs %zu bytes (16-byte aligned), got %zu", need,
+                ws ? ws_bytes : (size_t)0);
+  return hip_status(fa::launch_linear_bwd(*a, ws, static_cast<hipStream_t>(stream)),
+                    "fa_linear_bwd launch");
+}
+
+int fa_linear_decode(const fa_linear_decode_args* a, void* stream) {
+  const char* who = "fa_linear_decode";
+  if (!a) return fail(FA_E_INVALID, "%s: null args", who);
+  int st = check_linear(a, who);
+  if (st != FA_OK) return st;
+  if (a->num_states < 0) return fail(FA_E_INVALID, "%s: negative size", who);
+  st = check_rows(who, {a->q, a->k, a->v, a->out},
+                  {a->q_stride, a->k_stride, a->v_stride, a->o_stride}, 2);
+  if (st != FA_OK) return st;
+  if (!a->state) return fail(FA_E_INVALID, "%s: null state", who);
+  if ((st = check_state(who, a->state, a->s_stride)) != FA_OK) return st;
+  st = check_linear_grid(who, a->batch, a->num_heads, a->head_dim, 0);
+  if (st != FA_OK) return st;
+  if (a->batch == 0) return ok();
+  return hip_status(fa::launch_linear_decode(*a, static_cast<hipStream_t>(stream)),
+                    "fa_linear_decode launch");
 }
 
 }  // extern "C"

@@ -62,4 +62,18 @@ hipError_t noalloc_scratch(void** ptr);
 
 hipError_t launch_cache_write(const fa_cache_write_args& a, hipStream_t st);
 
+hipError_t launch_norm_rope(const fa_norm_rope_args& a, hipStream_t st);
+hipError_t launch_norm_rope_cache(const fa_norm_rope_cache_args& a, hipStream_t st);
+size_t norm_rope_bwd_workspace_bytes(const fa_norm_rope_bwd_args& a);
+hipError_t launch_norm_rope_bwd(const fa_norm_rope_bwd_args& a, void* ws, hipStream_t st);
+
+// linear_*_workgroups: workgroups of the widest launch's first grid dimension.
+int64_t linear_fwd_workgroups(const fa_linear_args& a);
+size_t linear_fwd_workspace_bytes(const fa_linear_args& a);
+hipError_t launch_linear_fwd(const fa_linear_args& a, void* ws, hipStream_t st);
+int64_t linear_bwd_workgroups(const fa_linear_bwd_args& a);
+size_t linear_bwd_workspace_bytes(const fa_linear_bwd_args& a);
+hipError_t launch_linear_bwd(const fa_linear_bwd_args& a, void* ws, hipStream_t st);
+hipError_t launch_linear_decode(const fa_linear_decode_args& a, hipStream_t st);
+
 }  // namespace fa

@@ -1,0 +1,874 @@
+// Linear attention with a decay for each head, forward and backward, on MFMA.
+//
+//   S_t = l S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t,   l = exp(log_decay[h]).
+//
+// Rows go in chunks of 64.  With S the state before a chunk of n rows,
+//   O  = scale ((Q K^T . M) V + diag(l^{i+1}) Q S),   M_ij = l^{i-j} (j <= i),
+//   S' = l^n S + sum_j l^{n-1-j} k_j v_j^T:
+// four matrix products a chunk instead of one rank-one update a row.
+//
+// The backward is the same operator three times:
+//   dq: (q, k, v) -> (dO, v, k), state transposed, time forward;
+//   dk: (v, dO, q) and dv: (k, q, dO), time reversed, where the carried state
+//   has its decay taken already (a row sees l^i of it instead of l^{i+1}, and
+//   the update's weights are l^{n-j}); its last value of the dv pass is the
+//   gradient of the initial state.
+// One kernel runs all of them ("passes"), in one launch.
+//
+// Work split: a workgroup holds one (sequence, head, segment)'s state in
+// registers and walks its chunks; each wave owns 32 of the state's columns (D / 32
+// waves).  Where sequences x heads are too few for the GPU, sequences are cut
+// into segments: one launch forms every segment's own state, one joins them in
+// order (linear_scan_kernel), and the main launch starts each segment from its
+// joined state.
+//
+// Registers and LDS: the state's accumulators (row d in the registers, column e
+// in the lane) are, rounded, the A operand of O^T = S^T Q^T as they stand: S never
+// leaves its registers.  The chunk's Q, K and V rows go through LDS; V^T and K^T
+// operands come from transposing LDS reads.
+//
+// Rounding: P = Q K^T . M and the copy of S that meets Q are rounded to the inputs'
+// type, once each, as the attention kernels round P.  The state itself is fp32,
+// and its update is kept exact to it: l^{n-1-j} v_j is split into NT terms of the
+// input type whose products with k are exact (three of bf16's 8 bits or two of
+// fp16's 11 make up fp32's 24).  fp16's terms would leave its range below 2^-14:
+// there a wave holds its columns of S times a power of two that keeps the largest
+// weighted value near 2^13, and takes it out at every use.
+#include "fa_common.h"
+#include "fa_fwd_d128.h"
+#include "fa_internal.h"
+
+namespace fa {
+
+namespace {
+
+constexpr int kChunk = 64;
+
+// One of q, k, v in a pass; head h of the pass reads head h / div.
+struct LinTensor {
+  const uint16_t* p;
+  int64_t s[3];  // batch, seq, head
+  int32_t div;
+};
+
+struct LinPass {
+  LinTensor q, k, v;
+  void* out;
+  int64_t os[3];
+  const float* init;  // [d][e] at d * ird + e * icd, nullptr: zero
+  float* fin;         // [d][e] contiguous, nullptr: not kept
+  int64_t is[2], fs[2];
+  int32_t ird, icd;
+  int32_t reverse, out_f32;
+  float p_scale, inter_scale, upd_scale;
+};
+
+struct LinParams {
+  LinPass pass[3];
+  const float* log_decay;
+  const int32_t* starts;  // packed form
+  const int32_t* prefix;
+  const int32_t* slots;
+  float* ws;  // [pass][slot][head][D][D]: the segments' states
+  int32_t batch, seqlen, heads, npass;
+  int32_t nseg;    // dense: segments of a sequence; packed: slots in all
+  int32_t seglen;  // rows of a segment, a multiple of kChunk
+  int32_t nstates;
+  int32_t segmented;
+};
+
+struct Segment {
+  int b, seg, nseg;  // sequence, segment, segments of the sequence; b < 0: none
+  int start, len;    // the sequence's first row and rows
+};
+
+// The packed sequence b, kept inside the rows there are whatever the offsets say.
+__device__ __forceinline__ void packed_rows(const LinParams& p, int b, int& start, int& len) {
+  const int s0 = min(max(p.starts[b], 0), p.seqlen);
+  const int s1 = min(max(p.starts[b + 1], s0), p.seqlen);
+  start = s0;
+  len = s1 - s0;
+}
+
+// Slot -> segment: dense slots are (sequence, segment); packed ones are handed
+// out in order, ceil(len / seglen) to a sequence, found by a wave scan.
+__device__ __forceinline__ Segment find_segment(const LinParams& p, int slot) {
+  Segment r;
+  if (!p.starts) {
+    r.b = slot / p.nseg;
+    r.seg = slot - r.b * p.nseg;
+    r.nseg = p.nseg;
+    r.start = 0;
+    r.len = p.seqlen;
+    if (r.seg * p.seglen >= r.len) r.b = -1;
+    return r;
+  }
+  r.b = -1;
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 64) {
+    const int b = b0 + lane;
+    int start = 0, len = 0;
+    if (b < p.batch) packed_rows(p, b, start, len);
+    const int n = (len + p.seglen - 1) / p.seglen;
+    const int end = base + wave_scan(n);
+    const uint64_t hit = __ballot(slot >= end - n && slot < end);
+    if (hit) {
+      const int src = __ffsll((unsigned long long)hit) - 1;
+      r.b = b0 + src;
+      r.nseg = __shfl(n, src);
+      r.seg = slot - (__shfl(end, src) - r.nseg);
+      r.start = __shfl(start, src);
+      r.len = __shfl(len, src);
+      break;
+    }
+    base = __shfl(end, 63);
+  }
+  r.b = __builtin_amdgcn_readfirstlane(r.b);
+  r.nseg = __builtin_amdgcn_readfirstlane(r.nseg);
+  r.seg = __builtin_amdgcn_readfirstlane(r.seg);
+  r.start = __builtin_amdgcn_readfirstlane(r.start);
+  r.len = __builtin_amdgcn_readfirstlane(r.len);
+  return r;
+}
+
+// The state slot of sequence b, or -1: it starts from zero and keeps nothing.
+__device__ __forceinline__ int state_slot(const LinParams& p, int b) {
+  const int s = p.slots ? p.slots[b] : b;
+  return s >= 0 && s < p.nstates ? s : -1;
+}
+__device__ __forceinline__ const float* init_of(const LinParams& p, const LinPass& a, int b, int h) {
+  const int s = state_slot(p, b);
+  if (!a.init || s < 0 || (p.prefix && p.prefix[b] <= 0)) return nullptr;
+  return a.init + s * a.is[0] + h * a.is[1];
+}
+__device__ __forceinline__ float* fin_of(const LinParams& p, const LinPass& a, int b, int h) {
+  const int s = state_slot(p, b);
+  return a.fin && s >= 0 ? a.fin + s * a.fs[0] + h * a.fs[1] : nullptr;
+}
+
+// log_decay[h], with -inf as a number whose product with 0 is 0.
+__device__ __forceinline__ float decay_of(const LinParams& p, int h) {
+  const float g = p.log_decay[h];
+  return g < -1e30f ? -1e30f : g;
+}
+
+template <int D>
+struct LinShape {
+  static constexpr int NW = D / 32;        // waves
+  static constexpr int THREADS = 64 * NW;
+  static constexpr int ROWB = 2 * D;       // bytes of a row in LDS
+  static constexpr int TILEB = kChunk * ROWB;
+  static constexpr int CPR = D / 8;        // 16-byte chunks of a row
+  static constexpr int DT = D / 32;        // 32-row tiles of the state
+};
+
+// LDS address of 16-byte chunk c of row r.
+template <int D>
+__device__ __forceinline__ int lds_at(int r, int c) {
+  return r * (2 * D) + ((c ^ swz_row<D>(r)) << 4);
+}
+
+// The chunk's rows of one tensor, 16 bytes x 4 a thread: row 16 u + tid / CPR.
+template <int D>
+struct Staged {
+  u32x4 x[4];
+};
+template <int D>
+__device__ __forceinline__ void load_rows(Staged<D>& s, const uint16_t* base, int64_t stride,
+                                          int first, int step, int n) {
+  using L = LinShape<D>;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int r = 16 * u + (int)threadIdx.x / L::CPR;
+    s.x[u] = u32x4{0, 0, 0, 0};
+    if (r < n)
+      s.x[u] = ld16(base + (int64_t)(first + step * r) * stride + 8 * (threadIdx.x % L::CPR));
+  }
+}
+template <int D>
+__device__ __forceinline__ void store_rows(const Staged<D>& s, char* lds) {
+  using L = LinShape<D>;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    st16(lds + lds_at<D>(16 * u + (int)threadIdx.x / L::CPR, threadIdx.x % L::CPR), s.x[u]);
+}
+
+// Operand with row or column 32 t + lr and k = 16 s + 8 lh + (0..7) from a
+// row-major [k][32 t + lr] tile in LDS.
+template <int D>
+__device__ __forceinline__ u32x4 read_transposed(const char* lds, int s, int t) {
+  const int lane = threadIdx.x & 63, i = lane & 15;
+  const int row = 16 * s + 8 * (lane >> 5) + (i >> 2);
+  const int col = 32 * t + (lane & 16) + 4 * (i & 3);
+  const u32x2 lo = lds_read_tr(lds + lds_at<D>(row, col >> 3) + 2 * (col & 7));
+  const u32x2 hi = lds_read_tr(lds + lds_at<D>(row + 4, col >> 3) + 2 * (col & 7));
+  return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// x as the sum of NT terms of the input type, each the rounding of what is left.
+template <class T, int NT>
+__device__ __forceinline__ void split_terms(float (&x)[8], u32x4 (&term)[NT]) {
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // One rounding for the term and for what is left of it: the compiler may
+      // otherwise round the product that x is to the term in one step, and x in
+      // two for the difference, which then differ by a whole step of the type.
+      asm("" : "+v"(x[2 * i]), "+v"(x[2 * i + 1]));
+      uint32_t w = T::pack(x[2 * i], x[2 * i + 1]);
+      asm("" : "+v"(w));
+      term[n][i] = w;
+      if (n + 1 < NT) {
+        x[2 * i] -= T::lo(w);
+        x[2 * i + 1] -= T::hi(w);
+      }
+    }
+}
+
+template <class T>
+constexpr int kTerms = T::kId == 0 ? 2 : 3;
+
+__device__ __forceinline__ float pow2(int e) {
+  return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23);
+}
+__device__ __forceinline__ int exponent(float x) {
+  return (int)((__builtin_bit_cast(uint32_t, x) >> 23) & 255) - 127;
+}
+
+// Exponent of the wave's largest |value| in fp16 words, or kNone where all are zero.
+constexpr int kNone = -1000;
+template <int N>
+__device__ __forceinline__ int max_exponent(const u32x4 (&w)[N]) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int s = 0; s < N; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[s][i] & 0x7fff7fffu));
+  const int top = wave_max_nonneg(max((int)m[0], (int)m[1]));
+  return top ? exponent(Half::lo((uint32_t)top)) : kNone;
+}
+
+// One segment of one head.  STATE_ONLY: forms the segment's own state (from
+// zero) into the workspace and no output.
+template <class T, int D, bool STATE_ONLY>
+__global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinParams p) {
+  using L = LinShape<D>;
+  constexpr int NT = kTerms<T>;
+  __shared__ __align__(16) char lds_q[STATE_ONLY ? 16 : L::TILEB];
+  __shared__ __align__(16) char lds_k[L::TILEB];
+  __shared__ __align__(16) char lds_v[L::TILEB];
+  __shared__ __align__(16) char lds_p[STATE_ONLY ? 16 : kChunk * 2 * kChunk];
+  __shared__ __align__(16) float weight[kChunk];  // of row j in the state's update
+
+  const int h = blockIdx.x % p.heads, slot = blockIdx.x / p.heads;
+  const LinPass& a = p.pass[blockIdx.y];
+  const Segment sg = find_segment(p, slot);
+  if (sg.b < 0) return;
+  float* fin = fin_of(p, a, sg.b, h);
+  const bool last = sg.seg == sg.nseg - 1;
+  if (STATE_ONLY && last && !fin) return;
+  const int row0 = sg.seg * p.seglen;
+  const int nrows = min(p.seglen, sg.len - row0);
+
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  const int lr = lane & 31, lh = lane >> 5;
+  const float g = decay_of(p, h), g2 = g * kLog2e;
+  const int sh = a.reverse ? 1 : 0;
+
+  const int batch = p.starts ? 0 : sg.b;
+  auto base_of = [&](const LinTensor& t) {
+    return t.p + batch * t.s[0] + (h / t.div) * t.s[2];
+  };
+  const uint16_t* qp = base_of(a.q);
+  const uint16_t* kp = base_of(a.k);
+  const uint16_t* vp = base_of(a.v);
+  const int step = a.reverse ? -1 : 1;
+  auto token = [&](int r) { return sg.start + (a.reverse ? sg.len - 1 - row0 - r : row0 + r); };
+
+  // State column 32 wave + lr, row 32 dt + 8 (i / 4) + 4 lh + i % 4.
+  f32x16 S[L::DT];
+  float* seg_state =
+      p.ws + (((int64_t)blockIdx.y * p.nseg * (p.starts ? 1 : p.batch) + slot) * p.heads + h) * D * D;
+  const int col = 32 * wave + lr;
+  {
+    const float* src = nullptr;
+    int ird = D, icd = 1;
+    if (!STATE_ONLY) {
+      if (p.segmented) {
+        src = seg_state;
+      } else {
+        src = init_of(p, a, sg.b, h);
+        ird = a.ird;
+        icd = a.icd;
+      }
+    }
+#pragma unroll
+    for (int dt = 0; dt < L::DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int d = 32 * dt + 8 * (i / 4) + 4 * lh + i % 4;
+        S[dt][i] = src ? src[d * ird + col * icd] : 0.f;
+      }
+  }
+
+  // P^T quadrants (32 keys j x 32 rows i) on and below the diagonal, dealt to the
+  // waves: 0 is (0, 0), 1 is (row tile 1, key tile 0), 2 is (1, 1).
+  constexpr int NQ = L::NW == 2 ? 2 : 1;
+  float pf[NQ][16];
+  if (!STATE_ONLY) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int quad = wave + L::NW * n;
+      const int row = 32 * (quad > 0) + lr;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = 32 * (quad > 1) + 8 * (i / 4) + 4 * lh + i % 4;
+        pf[n][i] = key <= row ? a.p_scale * fast_exp2(g2 * (float)(row - key)) : 0.f;
+      }
+    }
+  }
+  float rowf[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+    rowf[t] = a.inter_scale * fast_exp2(g2 * (float)(32 * t + lr + 1 - sh));
+
+  Staged<D> sq, sk, sv;
+  {
+    const int n = min(kChunk, nrows);
+    if (!STATE_ONLY) load_rows<D>(sq, qp, a.q.s[1], token(0), step, n);
+    load_rows<D>(sk, kp, a.k.s[1], token(0), step, n);
+    load_rows<D>(sv, vp, a.v.s[1], token(0), step, n);
+  }
+  int weights_n = 0;  // rows of the chunk that `weight` is for
+  int held = 0;       // S is held times 2^held (fp16)
+  // |weight| < 2^weight_top (upd_scale 0 or not finite: no scaling to speak of)
+  const int weight_top = min(max(exponent(a.upd_scale), -60), 60) + 1;
+
+  for (int c = 0; c < nrows; c += kChunk) {
+    const int n = min(kChunk, nrows - c);
+    __syncthreads();  // the last chunk's LDS reads are done
+    if (!STATE_ONLY) store_rows<D>(sq, lds_q);
+    store_rows<D>(sk, lds_k);
+    store_rows<D>(sv, lds_v);
+    if (n != weights_n) {
+      // Rows at or behind n are zeros: their weight only has to be finite.
+      if (threadIdx.x < kChunk)
+        weight[threadIdx.x] =
+            a.upd_scale * fast_exp2(g2 * (float)max(n - 1 - (int)threadIdx.x + sh, 0));
+      weights_n = n;
+    }
+    __syncthreads();
+    if (c + kChunk < nrows) {
+      const int m = min(kChunk, nrows - c - kChunk), t = token(c + kChunk);
+      if (!STATE_ONLY) load_rows<D>(sq, qp, a.q.s[1], t, step, m);
+      load_rows<D>(sk, kp, a.k.s[1], t, step, m);
+      load_rows<D>(sv, vp, a.v.s[1], t, step, m);
+    }
+
+    f32x16 o[2];
+    if constexpr (!STATE_ONLY) {
+      // P^T = K Q^T with the decay, rounded, as P's rows in LDS.
+#pragma unroll
+      for (int nq = 0; nq < NQ; ++nq) {
+        const int quad = wave + L::NW * nq;
+        if (quad < 3) {
+          const int it = quad > 0, jt = quad > 1;
+          f32x16 acc = {};
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            acc = T::mma32(ld16(lds_k + lds_at<D>(32 * jt + lr, 2 * kk + lh)),
+                           ld16(lds_q + lds_at<D>(32 * it + lr, 2 * kk + lh)), acc);
+#pragma unroll
+          for (int gi = 0; gi < 4; ++gi) {
+            u32x2 w;
+            w[0] = T::pack(acc[4 * gi] * pf[nq][4 * gi], acc[4 * gi + 1] * pf[nq][4 * gi + 1]);
+            w[1] = T::pack(acc[4 * gi + 2] * pf[nq][4 * gi + 2],
+                           acc[4 * gi + 3] * pf[nq][4 * gi + 3]);
+            st8(lds_p + lds_at<kChunk>(32 * it + lr, 4 * jt + gi) + 8 * lh, w);
+          }
+        }
+      }
+      // O^T = S^T Q^T, then the rows' decay.  fp16: S meets Q scaled by a power of
+      // two (its largest value to 2^14), so that neither a long memory's sums nor
+      // small ones leave the type's range.
+      float up = 1.f, down = 1.f;
+      if constexpr (T::kId == 0) {
+        float m = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < L::DT; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(S[dt][i]));
+        m = wave_max(m);
+        const int e = m > 0.f && m < __builtin_inff() ? min(max(exponent(m), -100), 100) : 14;
+        down = pow2(14 - e);
+        up = pow2(e - 14) * pow2(-held);
+      }
+      o[0] = o[1] = f32x16{};
+#pragma unroll
+      for (int dt = 0; dt < L::DT; ++dt)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          u32x4 sf;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sf[i] = T::pack(S[dt][8 * half + 2 * i] * down, S[dt][8 * half + 2 * i + 1] * down);
+#pragma unroll
+          for (int it = 0; it < 2; ++it) {
+            const u32x2 x = ld8(lds_q + lds_at<D>(32 * it + lr, 4 * dt + 2 * half) + 8 * lh);
+            const u32x2 y = ld8(lds_q + lds_at<D>(32 * it + lr, 4 * dt + 2 * half + 1) + 8 * lh);
+            o[it] = T::mma32(sf, u32x4{x[0], x[1], y[0], y[1]}, o[it]);
+          }
+        }
+#pragma unroll
+      for (int it = 0; it < 2; ++it)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[it][i] *= rowf[it] * up;
+      __syncthreads();  // P is there
+    }
+
+    // S = l^n S + K^T (weight V), and O^T += V^T P^T on the way.  The decay as
+    // S + S (l^n - 1): the factor's own rounding, which a slow decay would
+    // compound over hundreds of chunks, is then relative to the small difference.
+    {
+      const float dm1 = expm1f(g * (float)n);
+#pragma unroll
+      for (int dt = 0; dt < L::DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[dt][i] = fmaf(S[dt][i], dm1, S[dt][i]);
+    }
+    u32x4 vts[kChunk / 16];
+#pragma unroll
+    for (int s = 0; s < kChunk / 16; ++s) vts[s] = read_transposed<D>(lds_v, s, wave);
+    if constexpr (T::kId == 0) {
+      const int e = max_exponent(vts);
+      const int want = 13 - e - weight_top;
+      // Down where a term would overflow, up where eight bits would be lost.
+      if (e != kNone && (want < held || want > held + 8)) {
+        const float f = pow2(want - held);
+#pragma unroll
+        for (int dt = 0; dt < L::DT; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) S[dt][i] *= f;
+        held = want;
+      }
+    }
+    const float hold = T::kId == 0 ? pow2(held) : 1.f;
+#pragma unroll
+    for (int s = 0; s < kChunk / 16; ++s) {
+      const u32x4 vt = vts[s];
+      if constexpr (!STATE_ONLY) {
+#pragma unroll
+        for (int it = s / 2; it < 2; ++it)
+          o[it] = T::mma32(vt, ld16(lds_p + lds_at<kChunk>(32 * it + lr, 2 * s + lh)), o[it]);
+      }
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = T::lo(vt[i]) * (weight[16 * s + 8 * lh + 2 * i] * hold);
+        x[2 * i + 1] = T::hi(vt[i]) * (weight[16 * s + 8 * lh + 2 * i + 1] * hold);
+      }
+      u32x4 term[NT];
+      split_terms<T, NT>(x, term);
+#pragma unroll
+      for (int dt = 0; dt < L::DT; ++dt) {
+        const u32x4 kt = read_transposed<D>(lds_k, s, dt);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) S[dt] = T::mma32(kt, term[t], S[dt]);
+      }
+    }
+
+    if constexpr (!STATE_ONLY) {
+#pragma unroll
+      for (int it = 0; it < 2; ++it) {
+        const int r = 32 * it + lr;
+        if (r >= n) continue;
+        const int64_t at = batch * a.os[0] + token(c + r) * a.os[1] + h * a.os[2] + 32 * wave + 4 * lh;
+        if (a.out_f32) {
+          float* out = static_cast<float*>(a.out) + at;
+#pragma unroll
+          for (int gi = 0; gi < 4; ++gi)
+            *reinterpret_cast<f32x4*>(out + 8 * gi) =
+                f32x4{o[it][4 * gi], o[it][4 * gi + 1], o[it][4 * gi + 2], o[it][4 * gi + 3]};
+        } else {
+          uint16_t* out = static_cast<uint16_t*>(a.out) + at;
+#pragma unroll
+          for (int gi = 0; gi < 4; ++gi)
+            st8(out + 8 * gi, u32x2{T::pack(o[it][4 * gi], o[it][4 * gi + 1]),
+                                    T::pack(o[it][4 * gi + 2], o[it][4 * gi + 3])});
+        }
+      }
+    }
+  }
+
+  float* dst = STATE_ONLY ? seg_state : (p.segmented ? nullptr : fin);
+  if (!dst) return;
+#pragma unroll
+  for (int dt = 0; dt < L::DT; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      dst[(32 * dt + 8 * (i / 4) + 4 * lh + i % 4) * D + col] = S[dt][i] * pow2(-held);
+}
+
+// Joins the segments' states in order: each slot's own state becomes the state
+// before it, and the last sum the final state.  A thread holds four components.
+template <int D>
+__global__ __launch_bounds__(256) void linear_scan_kernel(LinParams p) {
+  constexpr int PARTS = D * D / 1024;
+  const int unit = blockIdx.x / PARTS, h = unit % p.heads, b = unit / p.heads;
+  const LinPass& a = p.pass[blockIdx.y];
+  const int at = 4 * ((int)(blockIdx.x % PARTS) * 256 + (int)threadIdx.x);
+  int first = b * p.nseg, len = p.seqlen;
+  if (p.starts) {
+    int start, n = 0;
+    const int lane = threadIdx.x & 63;
+    for (int i = lane; i < b; i += 64) {
+      packed_rows(p, i, start, len);
+      n += (len + p.seglen - 1) / p.seglen;
+    }
+    first = wave_total(n);
+    packed_rows(p, b, start, len);
+  }
+  const int64_t total = (int64_t)p.nseg * (p.starts ? 1 : p.batch);
+  // (Offsets that overlap would give more segments than there are slots.)
+  const int nseg = min((len + p.seglen - 1) / p.seglen, (int)max(total - first, (int64_t)0));
+  if (nseg == 0) return;
+  float* state = p.ws + ((blockIdx.y * total + first) * p.heads + h) * D * D + at;
+  const int64_t next = (int64_t)p.heads * D * D;
+  const float* init = init_of(p, a, b, h);
+  float* fin = fin_of(p, a, b, h);
+  const float g = decay_of(p, h);
+  const float dm1 = expm1f(g * (float)p.seglen);
+  f32x4 S = {0.f, 0.f, 0.f, 0.f};
+  if (init) {
+    const int d = at / D, e = at % D;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) S[i] = init[d * a.ird + (e + i) * a.icd];
+  }
+  for (int s = 0; s < nseg; ++s, state += next) {
+    f32x4 u = {0.f, 0.f, 0.f, 0.f};
+    if (s < nseg - 1 || fin) u = *reinterpret_cast<const f32x4*>(state);
+    *reinterpret_cast<f32x4*>(state) = S;
+    const float f = s < nseg - 1 ? dm1 : expm1f(g * (float)(len - s * p.seglen));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) S[i] = fmaf(S[i], f, S[i]) + u[i];
+  }
+  if (fin) *reinterpret_cast<f32x4*>(fin + at) = S;
+}
+
+// Gradients of shared heads: the fp32 parts of a KV head's query heads, in order.
+template <class T>
+__global__ __launch_bounds__(256) void linear_group_sum_kernel(const float* part, uint16_t* out,
+                                                               int64_t s0, int64_t s1, int64_t s2,
+                                                               int64_t total, int seqlen, int heads_k,
+                                                               int group, int D) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int cpr = D / 8;
+  const int c = (int)(i % cpr);
+  const int64_t row = i / cpr;  // (b, s, kv head)
+  const int hk = (int)(row % heads_k);
+  const int64_t t = row / heads_k;
+  const float* src = part + (row * group) * D + 8 * c;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+  for (int n = 0; n < group; ++n, src += D) {
+    x += *reinterpret_cast<const f32x4*>(src);
+    y += *reinterpret_cast<const f32x4*>(src + 4);
+  }
+  uint16_t* dst = out + (t / seqlen) * s0 + (t % seqlen) * s1 + hk * s2 + 8 * c;
+  st16(dst, u32x4{T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(y[0], y[1]),
+                  T::pack(y[2], y[3])});
+}
+
+// ------------------------------------------------------------------ decode
+
+// One token for each sequence: the state is read, updated and written once.
+// Bound by that memory (8 D^2 bytes a sequence and head; D^2 * 5 flops).  A
+// workgroup takes COLS columns of one head's state: every load is issued before
+// the first use, and a column's sum over d stays inside the workgroup.
+template <class T, int D, int COLS>
+__global__ __launch_bounds__(256) void linear_decode_kernel(fa_linear_decode_args a) {
+  constexpr int LANES = COLS / 4, ROWS = 256 / LANES, N = D / ROWS, SLICES = D / COLS;
+  __shared__ float qs[D], ks[D];
+  __shared__ __align__(16) float part[ROWS][COLS];
+  const int slice = blockIdx.x % SLICES;
+  const int h = (blockIdx.x / SLICES) % a.num_heads, b = blockIdx.x / SLICES / a.num_heads;
+  const int hk = h / (a.num_heads / a.num_heads_k);
+  const int slot = a.state_indices ? a.state_indices[b] : b;
+  const bool kept = slot >= 0 && slot < a.num_states;
+  const int e = slice * COLS + 4 * (threadIdx.x % LANES), r0 = threadIdx.x / LANES;
+  float* st = a.state + (kept ? slot * a.s_stride[0] + h * a.s_stride[1] : 0) + e;
+  f32x4 S[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    S[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (kept) S[i] = *reinterpret_cast<const f32x4*>(st + (r0 + i * ROWS) * D);
+  }
+  const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] + h * a.q_stride[1];
+  const uint16_t* k = static_cast<const uint16_t*>(a.k) + b * a.k_stride[0] + hk * a.k_stride[1];
+  const uint16_t* v = static_cast<const uint16_t*>(a.v) + b * a.v_stride[0] + hk * a.v_stride[1];
+  if (threadIdx.x < D) {
+    qs[threadIdx.x] = T::lo(q[threadIdx.x]);
+    ks[threadIdx.x] = T::lo(k[threadIdx.x]);
+  }
+  const u32x2 vw = ld8(v + e);
+  const f32x4 vv = {T::lo(vw[0]), T::hi(vw[0]), T::lo(vw[1]), T::hi(vw[1])};
+  const float decay = expf(a.log_decay[h]);
+  __syncthreads();
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int d = r0 + i * ROWS;
+    const float kd = ks[d], qd = qs[d];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      S[i][j] = fmaf(kd, vv[j], S[i][j] * decay);
+      o[j] = fmaf(qd, S[i][j], o[j]);
+    }
+    if (kept) *reinterpret_cast<f32x4*>(st + d * D) = S[i];
+  }
+  *reinterpret_cast<f32x4*>(&part[r0][4 * (threadIdx.x % LANES)]) = o;
+  __syncthreads();
+  if (threadIdx.x < COLS / 2) {
+    float x = 0.f, y = 0.f;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      x += part[r][2 * threadIdx.x];
+      y += part[r][2 * threadIdx.x + 1];
+    }
+    uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.o_stride[0] + h * a.o_stride[1];
+    *reinterpret_cast<uint32_t*>(out + slice * COLS + 2 * threadIdx.x) =
+        T::pack(x * a.scale, y * a.scale);
+  }
+}
+
+// ------------------------------------------------------------------ host
+
+// Rows of a segment: enough segments for every CU to hold two workgroups (four
+// of head_dim 64's half-size ones), none shorter than four chunks.
+int segment_rows(int64_t tokens, int64_t units, int D) {
+  const int64_t want = (int64_t)device_cu_count() * (D == 64 ? 4 : 2);
+  const int64_t n = units > 0 ? (want + units - 1) / units : 1;
+  int64_t rows = (tokens + n - 1) / n;
+  rows = (rows + kChunk - 1) / kChunk * kChunk;
+  return (int)std::max<int64_t>(rows, 4 * kChunk);
+}
+
+// Cuts p's sequences; returns the slots in all.
+int64_t set_segments(LinParams& p, int D) {
+  // Packed: the sequences' lengths are on the device; as if all were one.
+  const int64_t units = (int64_t)p.heads * p.npass * (p.starts ? 1 : p.batch);
+  p.seglen = segment_rows(p.seqlen, units, D);
+  p.segmented = p.seglen < p.seqlen;
+  if (p.starts) {
+    p.nseg = p.seqlen / p.seglen + p.batch;
+    return p.nseg;
+  }
+  p.nseg = (p.seqlen + p.seglen - 1) / p.seglen;
+  return (int64_t)p.nseg * p.batch;
+}
+
+size_t state_bytes(const LinParams& p, int64_t slots, int D) {
+  return p.segmented ? (size_t)slots * p.npass * p.heads * D * D * sizeof(float) : 0;
+}
+
+template <class T, int D>
+hipError_t launch_passes(LinParams& p, int64_t slots, hipStream_t st) {
+  using L = LinShape<D>;
+  const dim3 grid((unsigned)(slots * p.heads), p.npass);
+  if (p.segmented) {
+    hipLaunchKernelGGL((linear_kernel<T, D, true>), grid, dim3(L::THREADS), 0, st, p);
+    hipLaunchKernelGGL((linear_scan_kernel<D>), dim3((unsigned)(D * D / 1024 * p.batch * p.heads), p.npass),
+                       dim3(256), 0, st, p);
+  }
+  hipLaunchKernelGGL((linear_kernel<T, D, false>), grid, dim3(L::THREADS), 0, st, p);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_dim(LinParams& p, int64_t slots, int D, hipStream_t st) {
+  if (D == 64) return launch_passes<T, 64>(p, slots, st);
+  if (D == 128) return launch_passes<T, 128>(p, slots, st);
+  return launch_passes<T, 256>(p, slots, st);
+}
+
+LinTensor tensor(const void* x, const int64_t* s, int div) {
+  return {static_cast<const uint16_t*>(x), {s[0], s[1], s[2]}, div};
+}
+
+LinParams fwd_params(const fa_linear_args& a) {
+  LinParams p = {};
+  const int group = a.num_heads / a.num_heads_k, D = a.head_dim;
+  LinPass& f = p.pass[0];
+  f.q = tensor(a.q, a.q_stride, 1);
+  f.k = tensor(a.k, a.k_stride, group);
+  f.v = tensor(a.v, a.v_stride, group);
+  f.out = a.out;
+  for (int i = 0; i < 3; ++i) f.os[i] = a.o_stride[i];
+  f.init = a.initial_state;
+  f.fin = a.final_state;
+  for (int i = 0; i < 2; ++i) {
+    f.is[i] = a.is_stride[i];
+    f.fs[i] = a.fs_stride[i];
+  }
+  f.ird = D;
+  f.icd = 1;
+  f.p_scale = f.inter_scale = a.scale;
+  f.upd_scale = 1.f;
+  p.log_decay = a.log_decay;
+  p.starts = a.query_start_loc;
+  p.prefix = a.prefix_kv_lens;
+  p.slots = a.state_indices;
+  p.batch = a.batch;
+  p.seqlen = a.seqlen;
+  p.heads = a.num_heads;
+  p.npass = 1;
+  p.nstates = a.num_states;
+  return p;
+}
+
+LinParams bwd_params(const fa_linear_bwd_args& a) {
+  LinParams p = {};
+  const int group = a.num_heads / a.num_heads_k, D = a.head_dim;
+  const LinTensor q = tensor(a.q, a.q_stride, 1), k = tensor(a.k, a.k_stride, group);
+  const LinTensor v = tensor(a.v, a.v_stride, group), o = tensor(a.dout, a.do_stride, 1);
+  auto pass = [&](LinPass& f, const LinTensor& x, const LinTensor& y, const LinTensor& z, void* out,
+                  const int64_t* os, const float* init, const int64_t* is, bool transposed) {
+    f.q = x;
+    f.k = y;
+    f.v = z;
+    f.out = out;
+    for (int i = 0; i < 3; ++i) f.os[i] = os[i];
+    f.init = init;
+    for (int i = 0; i < 2; ++i) f.is[i] = is[i];
+    f.ird = transposed ? 1 : D;
+    f.icd = transposed ? D : 1;
+  };
+  pass(p.pass[0], o, v, k, a.dq, a.dq_stride, a.initial_state, a.is_stride, true);
+  p.pass[0].p_scale = p.pass[0].inter_scale = a.scale;
+  p.pass[0].upd_scale = 1.f;
+  pass(p.pass[1], v, o, q, a.dk, a.dk_stride, a.d_final_state, a.fs_stride, true);
+  pass(p.pass[2], k, q, o, a.dv, a.dv_stride, a.d_final_state, a.fs_stride, false);
+  for (int i = 1; i < 3; ++i) {
+    // The carried state holds the scale (the final state's gradient has none).
+    p.pass[i].reverse = 1;
+    p.pass[i].p_scale = p.pass[i].upd_scale = a.scale;
+    p.pass[i].inter_scale = 1.f;
+  }
+  p.pass[2].fin = a.d_initial_state;
+  for (int i = 0; i < 2; ++i) p.pass[2].fs[i] = a.dis_stride[i];
+  p.log_decay = a.log_decay;
+  p.batch = p.nstates = a.batch;
+  p.seqlen = a.seqlen;
+  p.heads = a.num_heads;
+  p.npass = 3;
+  return p;
+}
+
+// fp32 parts of dk and dv for each query head, where heads share k and v.
+size_t part_bytes(const fa_linear_bwd_args& a) {
+  return a.num_heads == a.num_heads_k
+             ? 0
+             : (size_t)a.batch * a.seqlen * a.num_heads * a.head_dim * sizeof(float);
+}
+
+template <class T, int D>
+hipError_t launch_decode_cols(const fa_linear_decode_args& a, hipStream_t st) {
+  // The fewest columns of a workgroup (32) while that leaves CUs without one.
+  constexpr int WIDE = D < 128 ? D : 128;
+  const int64_t heads = (int64_t)a.batch * a.num_heads;
+  if (heads * (D / WIDE) >= device_cu_count())
+    hipLaunchKernelGGL((linear_decode_kernel<T, D, WIDE>), dim3((unsigned)(heads * (D / WIDE))),
+                       dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((linear_decode_kernel<T, D, 32>), dim3((unsigned)(heads * (D / 32))),
+                       dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_decode_dim(const fa_linear_decode_args& a, hipStream_t st) {
+  if (a.head_dim == 64) return launch_decode_cols<T, 64>(a, st);
+  if (a.head_dim == 128) return launch_decode_cols<T, 128>(a, st);
+  return launch_decode_cols<T, 256>(a, st);
+}
+
+}  // namespace
+
+int64_t linear_fwd_workgroups(const fa_linear_args& a) {
+  LinParams p = fwd_params(a);
+  return set_segments(p, a.head_dim) * p.heads;
+}
+
+size_t linear_fwd_workspace_bytes(const fa_linear_args& a) {
+  LinParams p = fwd_params(a);
+  const int64_t slots = set_segments(p, a.head_dim);
+  return state_bytes(p, slots, a.head_dim);
+}
+
+hipError_t launch_linear_fwd(const fa_linear_args& a, void* ws, hipStream_t st) {
+  LinParams p = fwd_params(a);
+  const int64_t slots = set_segments(p, a.head_dim);
+  p.ws = static_cast<float*>(ws);
+  return a.dtype == FA_DTYPE_F16 ? launch_dim<Half>(p, slots, a.head_dim, st)
+                                 : launch_dim<BFloat16>(p, slots, a.head_dim, st);
+}
+
+int64_t linear_bwd_workgroups(const fa_linear_bwd_args& a) {
+  LinParams p = bwd_params(a);
+  return set_segments(p, a.head_dim) * p.heads;
+}
+
+size_t linear_bwd_workspace_bytes(const fa_linear_bwd_args& a) {
+  LinParams p = bwd_params(a);
+  const int64_t slots = set_segments(p, a.head_dim);
+  return state_bytes(p, slots, a.head_dim) + 2 * part_bytes(a);
+}
+
+hipError_t launch_linear_bwd(const fa_linear_bwd_args& a, void* ws, hipStream_t st) {
+  LinParams p = bwd_params(a);
+  const int64_t slots = set_segments(p, a.head_dim);
+  p.ws = static_cast<float*>(ws);
+  const size_t part = part_bytes(a);
+  float* dk = reinterpret_cast<float*>(static_cast<char*>(ws) + state_bytes(p, slots, a.head_dim));
+  float* dv = dk + part / sizeof(float);
+  if (part) {
+    for (int i = 1; i < 3; ++i) {
+      p.pass[i].out = i == 1 ? dk : dv;
+      p.pass[i].out_f32 = 1;
+      p.pass[i].os[2] = a.head_dim;
+      p.pass[i].os[1] = (int64_t)a.num_heads * a.head_dim;
+      p.pass[i].os[0] = p.pass[i].os[1] * a.seqlen;
+    }
+  }
+  const bool f16 = a.dtype == FA_DTYPE_F16;
+  hipError_t e = f16 ? launch_dim<Half>(p, slots, a.head_dim, st)
+                     : launch_dim<BFloat16>(p, slots, a.head_dim, st);
+  if (e != hipSuccess || !part) return e;
+  const int64_t total = (int64_t)a.batch * a.seqlen * a.num_heads_k * (a.head_dim / 8);
+  const dim3 grid((unsigned)((total + 255) / 256));
+  for (int i = 0; i < 2; ++i) {
+    const float* src = i ? dv : dk;
+    uint16_t* dst = static_cast<uint16_t*>(i ? a.dv : a.dk);
+    const int64_t* s = i ? a.dv_stride : a.dk_stride;
+    auto run = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, src, dst, s[0], s[1], s[2], total,
+                         a.seqlen, a.num_heads_k, a.num_heads / a.num_heads_k, a.head_dim);
+    };
+    if (f16)
+      run(linear_group_sum_kernel<Half>);
+    else
+      run(linear_group_sum_kernel<BFloat16>);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_linear_decode(const fa_linear_decode_args& a, hipStream_t st) {
+  return a.dtype == FA_DTYPE_F16 ? launch_decode_dim<Half>(a, st)
+                                 : launch_decode_dim<BFloat16>(a, st);
+}
+
+}  // namespace fa

@@ -34,6 +34,11 @@ struct Entries {
   decltype(&fa_paged_prefill_splitkv_workspace_bytes) paged_workspace;
   decltype(&fa_paged_prefill_splitkv) paged;
   decltype(&fa_reshape_and_cache) cache_write;
+  decltype(&fa_norm_rope) norm_rope;
+  decltype(&fa_norm_rope_and_cache) norm_rope_cache;
+  decltype(&fa_linear_fwd_workspace_bytes) linear_workspace;
+  decltype(&fa_linear_fwd) linear_fwd;
+  decltype(&fa_linear_decode) linear_decode;
 } lib;
 
 struct Call {
@@ -364,16 +369,290 @@ PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// bind(fa_fwd, fa_decode_workspace_bytes, fa_paged_decode, fa_paged_prefill_num_splits,
-//      fa_paged_prefill_splitkv_workspace_bytes, fa_paged_prefill_splitkv,
-//      fa_reshape_and_cache): the library's entry points, as addresses.
+// ------------------------------------------------------------------ norm and rotation
+
+bool same_half(const at::Tensor* t, const at::Tensor& like) {
+  return t && t->scalar_type() == like.scalar_type() && rows_ready(*t);
+}
+
+// Position tables, weights (None: no norm), eps and the pairing, which the
+// norm-and-rotation calls share.  `head` is a tensor [..., head_dim].
+template <class Args>
+bool rope_common(PyObject* cos_o, PyObject* sin_o, PyObject* qw_o, PyObject* kw_o, PyObject* eps,
+                 PyObject* interleaved, const at::Tensor& head, const Call& c, Args* p) {
+  const at::Tensor *cos = plain(cos_o, c, 2), *sin = plain(sin_o, c, 2);
+  if (!cos || !sin || cos->scalar_type() != at::kFloat || sin->scalar_type() != at::kFloat ||
+      cos->sizes() != sin->sizes() || cos->requires_grad() || sin->requires_grad())
+    return false;
+  const int64_t D = head.size(-1), R = 2 * cos->size(1);
+  if (D % 8 != 0 || D < 16 || D > 512 || R % 16 != 0 || R < 16 || R > D) return false;
+  const at::Tensor* tables[2] = {cos, sin};
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor& t = *tables[i];
+    p->table_stride[i] = t.size(0) == 1 ? 0 : t.stride(0);
+    if (t.stride(1) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0 ||
+        p->table_stride[i] < 0 || p->table_stride[i] % 4 != 0)
+      return false;
+  }
+  p->cos = cos->data_ptr<float>();
+  p->sin = sin->data_ptr<float>();
+  p->num_positions = cos->size(0);
+  PyObject* weights[2] = {qw_o, kw_o};
+  const void* ptr[2] = {nullptr, nullptr};
+  int f32 = -1;
+  for (int i = 0; i < 2; ++i) {
+    if (weights[i] == Py_None) continue;
+    const at::Tensor* w = plain(weights[i], c, 1);
+    if (!w || w->size(0) != D || !w->is_contiguous() ||
+        reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 != 0)
+      return false;
+    const int is32 = w->scalar_type() == at::kFloat;
+    if ((!is32 && w->scalar_type() != head.scalar_type()) || (f32 >= 0 && f32 != is32)) return false;
+    f32 = is32;
+    ptr[i] = w->data_ptr();
+  }
+  p->q_weight = ptr[0];
+  p->k_weight = ptr[1];
+  p->weight_f32 = f32 == 1;
+  if (interleaved != Py_True && interleaved != Py_False) return false;
+  p->interleaved = interleaved == Py_True;
+  p->head_dim = (int32_t)D;
+  p->rotary_dim = (int32_t)R;
+  return number(eps, &p->eps);
+}
+
+// int64 [n], contiguous, or nullptr.
+const int64_t* long_index(PyObject* o, const Call& c, int64_t n) {
+  const at::Tensor* t = plain(o, c, 1);
+  return t && t->scalar_type() == at::kLong && t->size(0) == n && t->is_contiguous()
+             ? t->data_ptr<int64_t>()
+             : nullptr;
+}
+
+// norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved, device, stream)
+//   -> (q_out, k_out) | status | None.  Positions: None or a vector.
+PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Call c;
+    fa_norm_rope_args p = {};
+    if (n != 11 || !call_of(a[9], a[10], &c)) return none();
+    const at::Tensor *q = plain(a[0], c, 4), *k = plain(a[1], c, 4);
+    const bool dense = q != nullptr;
+    if (!dense) {
+      q = plain(a[0], c, 3);
+      k = plain(a[1], c, 3);
+    }
+    if (!q || !k || !half_code(*q, &p.dtype) || !rows_ready(*q) || !same_half(k, *q) ||
+        !rope_common(a[2], a[3], a[4], a[5], a[7], a[8], *q, c, &p))
+      return none();
+    const int64_t d = q->dim();
+    for (int64_t i = 0; i < d; ++i)
+      if (i != d - 2 && q->size(i) != k->size(i)) return none();
+    for (int64_t i = 0; i < d; ++i)
+      if (!fits(q->size(i)) || !fits(k->size(i))) return none();
+    if (a[6] != Py_None) {
+      p.positions = long_index(a[6], c, q->size(d - 3));
+      if (!p.positions) return none();
+      p.pos_stride[1] = 1;
+    }
+    at::Tensor q_out, k_out;
+    int status;
+    {
+      NoGil no_gil;
+      q_out = at::empty(q->sizes(), q->options().requires_grad(false));
+      k_out = at::empty(k->sizes(), q_out.options());
+      p.q = q->data_ptr();
+      p.k = k->data_ptr();
+      p.q_out = q_out.data_ptr();
+      p.k_out = k_out.data_ptr();
+      auto put = [&](int64_t (&dst)[3], const at::Tensor& t) {
+        for (int64_t i = 0; i < d - 1; ++i)
+          dst[3 - (d - 1) + i] = t.size(i) == 1 ? 0 : t.stride(i);
+      };
+      put(p.q_stride, *q);
+      put(p.k_stride, *k);
+      put(p.qo_stride, q_out);
+      put(p.ko_stride, k_out);
+      p.batch = dense ? (int32_t)q->size(0) : 1;
+      p.seqlen = (int32_t)q->size(d - 3);
+      p.num_heads = (int32_t)q->size(d - 2);
+      p.num_heads_k = (int32_t)k->size(d - 2);
+      status = lib.norm_rope(&p, c.stream);
+    }
+    if (status != FA_OK) return PyLong_FromLong(status);
+    return Py_BuildValue("NN", THPVariable_Wrap(q_out), THPVariable_Wrap(k_out));
+  });
+}
+
+// norm_rope_cache(q, k, v, key_cache, value_cache, slot_mapping, positions, cos, sin,
+//                 q_weight, k_weight, eps, interleaved, device, stream) -> q_out | status | None
+PyObject* norm_rope_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Call c;
+    fa_norm_rope_cache_args p = {};
+    if (n != 15 || !call_of(a[13], a[14], &c)) return none();
+    const at::Tensor *q = plain(a[0], c, 3), *k = plain(a[1], c, 3), *v = plain(a[2], c, 3),
+                     *kc = plain(a[3], c, 4), *vc = plain(a[4], c, 4);
+    if (!q || !half_code(*q, &p.dtype) || !rows_ready(*q) || !same_half(k, *q) ||
+        !same_half(v, *q) || !same_half(kc, *q) || !same_half(vc, *q) ||
+        k->sizes() != v->sizes() || kc->sizes() != vc->sizes() || kc->size(2) != k->size(1) ||
+        kc->size(3) != k->size(2) || q->size(0) != k->size(0) || q->size(2) != k->size(2) ||
+        !fits(q->size(0)) || !fits(q->size(1)) || !fits(k->size(1)) || !fits(kc->size(0)) ||
+        !fits(kc->size(1)) ||
+        !rope_common(a[7], a[8], a[9], a[10], a[11], a[12], *q, c, &p))
+      return none();
+    p.slot_mapping = long_index(a[5], c, q->size(0));
+    p.positions = long_index(a[6], c, q->size(0));
+    if (!p.slot_mapping || !p.positions) return none();
+    at::Tensor out;
+    int status;
+    {
+      NoGil no_gil;
+      out = at::empty(q->sizes(), q->options().requires_grad(false));
+      p.q = q->data_ptr();
+      p.k = k->data_ptr();
+      p.v = v->data_ptr();
+      p.q_out = out.data_ptr();
+      p.k_cache = kc->data_ptr();
+      p.v_cache = vc->data_ptr();
+      set_strides(p.q_stride, *q);
+      set_strides(p.key_stride, *k);
+      set_strides(p.value_stride, *v);
+      set_strides(p.qo_stride, out);
+      set_strides(p.k_stride, *kc);
+      set_strides(p.v_stride, *vc);
+      p.num_tokens = (int32_t)q->size(0);
+      p.num_heads = (int32_t)q->size(1);
+      p.num_kv_heads = (int32_t)k->size(1);
+      p.num_pages = (int32_t)kc->size(0);
+      p.page_size = (int32_t)kc->size(1);
+      status = lib.norm_rope_cache(&p, c.stream);
+    }
+    if (status != FA_OK) return PyLong_FromLong(status);
+    return THPVariable_Wrap(out);
+  });
+}
+
+// ------------------------------------------------------------------ linear attention
+
+// q [n, H, D], k, v [n, Hk, D], log_decay [H], a state pool [N, H, D, D], slots
+// (None or int32 [batch]) and the scale, of the serving calls.  `batch`: sequences.
+template <class Args>
+bool linear_common(PyObject* const* a, PyObject* slots_o, PyObject* scale, int64_t batch,
+                   const Call& c, const at::Tensor* q, Args* p, const at::Tensor** state) {
+  const at::Tensor *k = plain(a[1], c, 3), *v = plain(a[2], c, 3), *g = plain(a[3], c, 1),
+                   *s = plain(a[4], c, 4);
+  if (!half_code(*q, &p->dtype) || !rows_ready(*q) || !same_half(k, *q) || !same_half(v, *q) ||
+      k->sizes() != v->sizes() || k->size(0) != q->size(0) || k->size(2) != q->size(2) || !g || !s)
+    return false;
+  const int64_t H = q->size(1), Hk = k->size(1), D = q->size(2);
+  if ((D != 64 && D != 128 && D != 256) || H % Hk != 0 || !fits(H) || !fits(q->size(0)) ||
+      g->scalar_type() != at::kFloat || g->size(0) != H || !g->is_contiguous() ||
+      g->requires_grad() || s->scalar_type() != at::kFloat || s->size(1) != H ||
+      s->size(2) != D || s->size(3) != D || !fits(s->size(0)) || !s->is_contiguous() ||
+      reinterpret_cast<uintptr_t>(s->data_ptr()) % 16 != 0 || !scale_of(scale, D, &p->scale))
+    return false;
+  if (slots_o != Py_None) {
+    const at::Tensor* slots = plain(slots_o, c, 1);
+    if (!index_ready(slots) || slots->size(0) != batch) return false;
+    p->state_indices = slots->data_ptr<int32_t>();
+  } else if (batch > s->size(0)) {
+    return false;
+  }
+  p->q = q->data_ptr();
+  p->k = k->data_ptr();
+  p->v = v->data_ptr();
+  p->log_decay = g->data_ptr<float>();
+  p->num_heads = (int32_t)H;
+  p->num_heads_k = (int32_t)Hk;
+  p->head_dim = (int32_t)D;
+  p->num_states = (int32_t)s->size(0);
+  p->batch = (int32_t)batch;
+  *state = s;
+  return true;
+}
+
+// linear_prefill(q, k, v, log_decay, state, query_start_loc, prefix_kv_lens, state_indices,
+//                scale, device, stream) -> out | status | None
+PyObject* linear_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Call c;
+    fa_linear_args p = {};
+    if (n != 11 || !call_of(a[9], a[10], &c)) return none();
+    const at::Tensor *q = plain(a[0], c, 3), *starts = plain(a[5], c, 1),
+                     *prefix = plain(a[6], c, 1), *state = nullptr;
+    if (!q || !index_ready(starts) || !index_ready(prefix) ||
+        starts->size(0) != prefix->size(0) + 1 || !fits(prefix->size(0)) ||
+        !linear_common(a, a[7], a[8], prefix->size(0), c, q, &p, &state))
+      return none();
+    const at::Tensor &k = THPVariable_Unpack(a[1]), &v = THPVariable_Unpack(a[2]);
+    at::Tensor out;
+    int status;
+    {
+      NoGil no_gil;
+      out = at::empty(q->sizes(), q->options().requires_grad(false));
+      auto put = [](int64_t (&dst)[3], const at::Tensor& t) {
+        dst[1] = t.size(0) == 1 ? 0 : t.stride(0);
+        dst[2] = t.size(1) == 1 ? 0 : t.stride(1);
+      };
+      put(p.q_stride, *q);
+      put(p.k_stride, k);
+      put(p.v_stride, v);
+      put(p.o_stride, out);
+      p.out = out.data_ptr();
+      p.initial_state = p.final_state = state->data_ptr<float>();
+      set_strides(p.is_stride, *state);
+      set_strides(p.fs_stride, *state);
+      p.query_start_loc = starts->data_ptr<int32_t>();
+      p.prefix_kv_lens = prefix->data_ptr<int32_t>();
+      p.seqlen = (int32_t)q->size(0);
+      const size_t bytes = lib.linear_workspace(&p);
+      at::Tensor ws;
+      if (bytes) ws = at::empty({(int64_t)bytes}, out.options().dtype(at::kByte));
+      status = lib.linear_fwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, c.stream);
+    }
+    if (status != FA_OK) return PyLong_FromLong(status);
+    return THPVariable_Wrap(out);
+  });
+}
+
+// linear_decode(q, k, v, log_decay, state, state_indices, scale, device, stream)
+//   -> out | status | None
+PyObject* linear_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Call c;
+    fa_linear_decode_args p = {};
+    if (n != 9 || !call_of(a[7], a[8], &c)) return none();
+    const at::Tensor *q = plain(a[0], c, 3), *state = nullptr;
+    if (!q || !linear_common(a, a[5], a[6], q->size(0), c, q, &p, &state)) return none();
+    at::Tensor out;
+    int status;
+    {
+      NoGil no_gil;
+      out = at::empty(q->sizes(), q->options().requires_grad(false));
+      set_strides(p.q_stride, *q);
+      set_strides(p.k_stride, THPVariable_Unpack(a[1]));
+      set_strides(p.v_stride, THPVariable_Unpack(a[2]));
+      set_strides(p.o_stride, out);
+      set_strides(p.s_stride, *state);
+      p.out = out.data_ptr();
+      p.state = state->data_ptr<float>();
+      status = lib.linear_decode(&p, c.stream);
+    }
+    if (status != FA_OK) return PyLong_FromLong(status);
+    return THPVariable_Wrap(out);
+  });
+}
+
+// bind(...): the library's entry points, as addresses, in the order of Entries.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void* f[7];
-  if (n != 7) {
-    PyErr_SetString(PyExc_TypeError, "bind takes seven addresses");
+  constexpr int kEntries = 12;
+  void* f[kEntries];
+  if (n != kEntries) {
+    PyErr_Format(PyExc_TypeError, "bind takes %d addresses", kEntries);
     return nullptr;
   }
-  for (int i = 0; i < 7; ++i) {
+  for (int i = 0; i < kEntries; ++i) {
     f[i] = PyLong_AsVoidPtr(a[i]);
     if (PyErr_Occurred()) return nullptr;
   }
@@ -383,7 +662,12 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
          reinterpret_cast<decltype(lib.paged_splits)>(f[3]),
          reinterpret_cast<decltype(lib.paged_workspace)>(f[4]),
          reinterpret_cast<decltype(lib.paged)>(f[5]),
-         reinterpret_cast<decltype(lib.cache_write)>(f[6])};
+         reinterpret_cast<decltype(lib.cache_write)>(f[6]),
+         reinterpret_cast<decltype(lib.norm_rope)>(f[7]),
+         reinterpret_cast<decltype(lib.norm_rope_cache)>(f[8]),
+         reinterpret_cast<decltype(lib.linear_workspace)>(f[9]),
+         reinterpret_cast<decltype(lib.linear_fwd)>(f[10]),
+         reinterpret_cast<decltype(lib.linear_decode)>(f[11])};
   Py_RETURN_NONE;
 }
 
@@ -398,6 +682,10 @@ PyMethodDef methods[] = {method<bind>("bind"),
                          method<decode>("decode"),
                          method<paged_forward>("paged_forward"),
                          method<cache_write>("cache_write"),
+                         method<norm_rope>("norm_rope"),
+                         method<norm_rope_cache>("norm_rope_cache"),
+                         method<linear_prefill>("linear_prefill"),
+                         method<linear_decode>("linear_decode"),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_fa_torch", nullptr, -1, methods};

@@ -104,6 +104,84 @@ class CacheWriteArgs(ctypes.Structure):
     ]
 
 
+class NormRopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("q_out", _vp), ("k_out", _vp),
+        ("q_weight", _vp), ("k_weight", _vp), ("cos", _vp), ("sin", _vp), ("positions", _vp),
+        ("q_stride", _i64x3), ("k_stride", _i64x3), ("qo_stride", _i64x3),
+        ("ko_stride", _i64x3), ("table_stride", _i64x2), ("pos_stride", _i64x2),
+        ("num_positions", ctypes.c_int64),
+        ("batch", _i32), ("seqlen", _i32), ("num_heads", _i32), ("num_heads_k", _i32),
+        ("head_dim", _i32), ("rotary_dim", _i32), ("interleaved", _i32), ("weight_f32", _i32),
+        ("dtype", _i32), ("eps", _f32),
+    ]
+
+
+class NormRopeBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("dq_out", _vp), ("dk_out", _vp), ("dq", _vp), ("dk", _vp),
+        ("q_weight", _vp), ("k_weight", _vp), ("dq_weight", _vp), ("dk_weight", _vp),
+        ("cos", _vp), ("sin", _vp), ("positions", _vp),
+        ("q_stride", _i64x3), ("k_stride", _i64x3), ("dqo_stride", _i64x3),
+        ("dko_stride", _i64x3), ("dq_stride", _i64x3), ("dk_stride", _i64x3),
+        ("table_stride", _i64x2), ("pos_stride", _i64x2), ("num_positions", ctypes.c_int64),
+        ("batch", _i32), ("seqlen", _i32), ("num_heads", _i32), ("num_heads_k", _i32),
+        ("head_dim", _i32), ("rotary_dim", _i32), ("interleaved", _i32), ("weight_f32", _i32),
+        ("dtype", _i32), ("eps", _f32),
+    ]
+
+
+class NormRopeCacheArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("q_out", _vp), ("k_cache", _vp), ("v_cache", _vp),
+        ("slot_mapping", _vp), ("positions", _vp), ("q_weight", _vp), ("k_weight", _vp),
+        ("cos", _vp), ("sin", _vp),
+        ("q_stride", _i64x2), ("key_stride", _i64x2), ("value_stride", _i64x2),
+        ("qo_stride", _i64x2), ("k_stride", _i64x3), ("v_stride", _i64x3),
+        ("table_stride", _i64x2), ("num_positions", ctypes.c_int64),
+        ("num_tokens", _i32), ("num_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+        ("rotary_dim", _i32), ("page_size", _i32), ("num_pages", _i32), ("interleaved", _i32),
+        ("weight_f32", _i32), ("dtype", _i32), ("eps", _f32),
+    ]
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("log_decay", _vp),
+        ("initial_state", _vp), ("final_state", _vp), ("query_start_loc", _vp),
+        ("prefix_kv_lens", _vp), ("state_indices", _vp),
+        ("q_stride", _i64x3), ("k_stride", _i64x3), ("v_stride", _i64x3), ("o_stride", _i64x3),
+        ("is_stride", _i64x2), ("fs_stride", _i64x2),
+        ("batch", _i32), ("seqlen", _i32), ("num_heads", _i32), ("num_heads_k", _i32),
+        ("head_dim", _i32), ("num_states", _i32), ("scale", _f32), ("dtype", _i32),
+    ]
+
+
+class LinearBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("dout", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
+        ("log_decay", _vp), ("initial_state", _vp), ("d_final_state", _vp),
+        ("d_initial_state", _vp),
+        ("q_stride", _i64x3), ("k_stride", _i64x3), ("v_stride", _i64x3),
+        ("do_stride", _i64x3), ("dq_stride", _i64x3), ("dk_stride", _i64x3),
+        ("dv_stride", _i64x3), ("is_stride", _i64x2), ("fs_stride", _i64x2),
+        ("dis_stride", _i64x2),
+        ("batch", _i32), ("seqlen", _i32), ("num_heads", _i32), ("num_heads_k", _i32),
+        ("head_dim", _i32), ("scale", _f32), ("dtype", _i32),
+    ]
+
+
+class LinearDecodeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("log_decay", _vp), ("state", _vp),
+        ("state_indices", _vp),
+        ("q_stride", _i64x2), ("k_stride", _i64x2), ("v_stride", _i64x2), ("o_stride", _i64x2),
+        ("s_stride", _i64x2),
+        ("batch", _i32), ("num_heads", _i32), ("num_heads_k", _i32), ("head_dim", _i32),
+        ("num_states", _i32), ("scale", _f32), ("dtype", _i32),
+    ]
+
+
 # Every function the header declares, with its ctypes prototype.
 _PROTOTYPES = {
     "fa_abi_version": (ctypes.c_int, []),
@@ -124,6 +202,16 @@ _PROTOTYPES = {
     "fa_paged_decode": (ctypes.c_int, [ctypes.POINTER(DecodeArgs), _vp, ctypes.c_size_t, _vp]),
     "fa_paged_decode_noalloc": (ctypes.c_int, [ctypes.POINTER(DecodeArgs), _vp]),
     "fa_reshape_and_cache": (ctypes.c_int, [ctypes.POINTER(CacheWriteArgs), _vp]),
+    "fa_norm_rope": (ctypes.c_int, [ctypes.POINTER(NormRopeArgs), _vp]),
+    "fa_norm_rope_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(NormRopeBwdArgs)]),
+    "fa_norm_rope_bwd": (ctypes.c_int, [ctypes.POINTER(NormRopeBwdArgs), _vp, ctypes.c_size_t,
+                                        _vp]),
+    "fa_norm_rope_and_cache": (ctypes.c_int, [ctypes.POINTER(NormRopeCacheArgs), _vp]),
+    "fa_linear_fwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LinearArgs)]),
+    "fa_linear_fwd": (ctypes.c_int, [ctypes.POINTER(LinearArgs), _vp, ctypes.c_size_t, _vp]),
+    "fa_linear_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LinearBwdArgs)]),
+    "fa_linear_bwd": (ctypes.c_int, [ctypes.POINTER(LinearBwdArgs), _vp, ctypes.c_size_t, _vp]),
+    "fa_linear_decode": (ctypes.c_int, [ctypes.POINTER(LinearDecodeArgs), _vp]),
 }
 
 _lock = threading.Lock()

@@ -19,7 +19,9 @@ from . import _lib
 
 _ENTRIES = ("fa_fwd", "fa_decode_workspace_bytes", "fa_paged_decode",
             "fa_paged_prefill_num_splits", "fa_paged_prefill_splitkv_workspace_bytes",
-            "fa_paged_prefill_splitkv", "fa_reshape_and_cache")
+            "fa_paged_prefill_splitkv", "fa_reshape_and_cache", "fa_norm_rope",
+            "fa_norm_rope_and_cache", "fa_linear_fwd_workspace_bytes", "fa_linear_fwd",
+            "fa_linear_decode")
 _lock = threading.Lock()
 _module = None
 _missing = False  # load() failed: the Python path takes every call
@@ -101,3 +103,23 @@ def paged_forward(q, k_cache, v_cache, block_table, seq_lens, query_start_loc, p
 def cache_write(key, *args):
     """0, or None."""
     return _run("cache_write", "fa_reshape_and_cache", key, (key, *args))
+
+
+def norm_rope(q, *args):
+    """(q_out, k_out), or None."""
+    return _run("norm_rope", "fa_norm_rope", q, (q, *args))
+
+
+def norm_rope_cache(q, *args):
+    """q_out, or None."""
+    return _run("norm_rope_cache", "fa_norm_rope_and_cache", q, (q, *args))
+
+
+def linear_prefill(q, *args):
+    """out, or None."""
+    return _run("linear_prefill", "fa_linear_fwd", q, (q, *args))
+
+
+def linear_decode(q, *args):
+    """out, or None."""
+    return _run("linear_decode", "fa_linear_decode", q, (q, *args))
