@@ -473,7 +473,7 @@ int fa_norm_rope_and_cache(const fa_norm_rope_cache_args* args, void* stream);
 /* log_decay fp32 [num_heads], natural log, <= 0 (-inf: no memory).         */
 /*   dense (query_start_loc NULL): q, out [batch, seqlen, num_heads,        */
 /*     head_dim], k, v [batch, seqlen, num_heads_k, head_dim] (strides      */
-/*     {batch, seq, head});                                                 */
+/*     {batch, seq, head}, sequence strides below 2^24);                    */
 /*   packed: the same with one batch of num_tokens rows (the batch strides  */
 /*     are not read); sequence b is rows query_start_loc[b] ..              */
 /*     query_start_loc[b + 1] - 1, rows of no sequence stay as they were.   */

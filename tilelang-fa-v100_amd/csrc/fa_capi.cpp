@@ -527,6 +527,14 @@ static int check_state(const char* who, const float* s, const int64_t (&stride)[
   return ok();
 }
 
+// The kernels address a chunk's 64 rows with 32-bit byte offsets, fp32 ones among them.
+static int check_row_strides(const char* who, std::initializer_list<const int64_t*> strides) {
+  for (const int64_t* s : strides)
+    if (s[1] >= kMaxFwdKvRowStride)
+      return fail(FA_E_UNSUPPORTED, "%s: sequence strides must be below 2^24 elements", who);
+  return ok();
+}
+
 // Workgroups of one launch: sequences x heads x up to 64 parts of a state, and
 // the segments.
 static int check_linear_grid(const char* who, int64_t batch, int heads, int D, int64_t groups) {
@@ -543,6 +551,8 @@ static int check_linear_fwd(const fa_linear_args* a) {
   if (a->seqlen < 0 || a->num_states < 0) return fail(FA_E_INVALID, "%s: negative size", who);
   st = check_rows(who, {a->q, a->k, a->v, a->out},
                   {a->q_stride, a->k_stride, a->v_stride, a->o_stride}, 3);
+  if (st != FA_OK) return st;
+  st = check_row_strides(who, {a->q_stride, a->k_stride, a->v_stride, a->o_stride});
   if (st != FA_OK) return st;
   if ((st = check_state(who, a->initial_state, a->is_stride)) != FA_OK) return st;
   if ((st = check_state(who, a->final_state, a->fs_stride)) != FA_OK) return st;
@@ -580,6 +590,12 @@ static int check_linear_bwd(const fa_linear_bwd_args* a) {
                   {a->q_stride, a->k_stride, a->v_stride, a->do_stride, a->dq_stride,
                    a->dk_stride, a->dv_stride}, 3);
   if (st != FA_OK) return st;
+  st = check_row_strides(who, {a->q_stride, a->k_stride, a->v_stride, a->do_stride, a->dq_stride,
+                               a->dk_stride, a->dv_stride});
+  if (st != FA_OK) return st;
+  // (Shared heads: fp32 rows of all query heads.)
+  if ((int64_t)a->num_heads * a->head_dim >= kMaxFwdKvRowStride)
+    return fail(FA_E_UNSUPPORTED, "%s: problem too large", who);
   if ((st = check_state(who, a->initial_state, a->is_stride)) != FA_OK) return st;
   if ((st = check_state(who, a->d_final_state, a->fs_stride)) != FA_OK) return st;
   if ((st = check_state(who, a->d_initial_state, a->dis_stride)) != FA_OK) return st;

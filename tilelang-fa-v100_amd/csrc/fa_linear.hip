@@ -31,7 +31,9 @@
 // type, once each, as the attention kernels round P.  The state itself is fp32,
 // and its update is kept exact to it: l^{n-1-j} v_j is split into NT terms of the
 // input type whose products with k are exact (three of bf16's 8 bits or two of
-// fp16's 11 make up fp32's 24).  fp16's terms would leave its range below 2^-14:
+// fp16's 11 make up fp32's 24; two of bf16's, where no state is returned, were 2%
+// faster at head_dim 128, and outputs would then differ with what is asked for).
+// fp16's terms would leave its range below 2^-14:
 // there a wave holds its columns of S times a power of two that keeps the largest
 // weighted value near 2^13, and takes it out at every use.
 #include "fa_common.h"
@@ -153,57 +155,86 @@ __device__ __forceinline__ float decay_of(const LinParams& p, int h) {
   return g < -1e30f ? -1e30f : g;
 }
 
+// LDS rows of `W` 16-bit elements.  Rows are 64 bytes (16 banks) apart in bank
+// terms and every fourth row 16 bytes further, so that the operand reads (16 bytes
+// of 16 rows) and the transposing reads (64 bytes of 4 rows) each touch every bank
+// once, with addresses that are one lane register plus an immediate: with an XOR
+// swizzle instead the compiler held some 40 address registers and spilled.
+template <int W>
+struct Rows16 {
+  static constexpr int kStride = 2 * W + 64;
+  static constexpr int kBytes = kChunk * kStride + kChunk / 4 * 16;
+  __device__ static __forceinline__ int at(int r) { return r * kStride + (r >> 2) * 16; }
+};
+
 template <int D>
 struct LinShape {
   static constexpr int NW = D / 32;        // waves
   static constexpr int THREADS = 64 * NW;
-  static constexpr int ROWB = 2 * D;       // bytes of a row in LDS
-  static constexpr int TILEB = kChunk * ROWB;
   static constexpr int CPR = D / 8;        // 16-byte chunks of a row
   static constexpr int DT = D / 32;        // 32-row tiles of the state
+  using Tile = Rows16<D>;
+  using Scores = Rows16<kChunk>;
 };
 
-// LDS address of 16-byte chunk c of row r.
-template <int D>
-__device__ __forceinline__ int lds_at(int r, int c) {
-  return r * (2 * D) + ((c ^ swz_row<D>(r)) << 4);
-}
+// Q and K rows are kept with their 4-element groups in the order 0, 2, 1, 3 of
+// each 16: lane half lh then finds the 8 components that the state's accumulators
+// give it (4 lh + 0..3 and 8 + 4 lh + 0..3) in one 16-byte read.
+__device__ __forceinline__ int group_at(int g) { return 8 * ((g & 1) * 2 + (g >> 1)); }
 
-// The chunk's rows of one tensor, 16 bytes x 4 a thread: row 16 u + tid / CPR.
+// A chunk's rows of one tensor on the way to LDS, 16 bytes x 4 a thread: row
+// 16 u + tid / CPR.  Rows at or behind n are zeros.
 template <int D>
 struct Staged {
   u32x4 x[4];
 };
+// `lowest`: the chunk's row with the lowest address; rows go up from it (step 1)
+// or down to it from row 0 (step -1).
 template <int D>
-__device__ __forceinline__ void load_rows(Staged<D>& s, const uint16_t* base, int64_t stride,
-                                          int first, int step, int n) {
+__device__ __forceinline__ void load_rows(Staged<D>& s, const uint16_t* lowest, int64_t stride,
+                                          int step, int n) {
   using L = LinShape<D>;
+  const rsrc_t rs = make_rsrc(lowest, (uint32_t)((n - 1) * stride + D) * 2u);
+  const int r0 = (int)threadIdx.x / L::CPR;
+  const uint32_t row = 2 * (uint32_t)stride;  // bytes
+  const uint32_t at = 16 * (threadIdx.x % L::CPR);
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    const int r = 16 * u + (int)threadIdx.x / L::CPR;
-    s.x[u] = u32x4{0, 0, 0, 0};
-    if (r < n)
-      s.x[u] = ld16(base + (int64_t)(first + step * r) * stride + 8 * (threadIdx.x % L::CPR));
+    const int r = 16 * u + r0;
+    const uint32_t off = (uint32_t)(step > 0 ? r : n - 1 - r) * row + at;
+    s.x[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, r < n ? off : 0xffffffffu, 0, 0);
   }
 }
-template <int D>
+template <int D, bool GROUPED>
 __device__ __forceinline__ void store_rows(const Staged<D>& s, char* lds) {
   using L = LinShape<D>;
+  const int r0 = (int)threadIdx.x / L::CPR, c = threadIdx.x % L::CPR;
+  char* p = lds + L::Tile::at(r0) + (GROUPED ? 32 * (c >> 1) + 8 * (c & 1) : 16 * c);
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
-    st16(lds + lds_at<D>(16 * u + (int)threadIdx.x / L::CPR, threadIdx.x % L::CPR), s.x[u]);
+  for (int u = 0; u < 4; ++u, p += L::Tile::at(16)) {
+    if constexpr (GROUPED) {
+      st8(p, u32x2{s.x[u][0], s.x[u][1]});
+      st8(p + 16, u32x2{s.x[u][2], s.x[u][3]});
+    } else {
+      st16(p, s.x[u]);
+    }
+  }
 }
 
-// Operand with row or column 32 t + lr and k = 16 s + 8 lh + (0..7) from a
-// row-major [k][32 t + lr] tile in LDS.
-template <int D>
-__device__ __forceinline__ u32x4 read_transposed(const char* lds, int s, int t) {
-  const int lane = threadIdx.x & 63, i = lane & 15;
-  const int row = 16 * s + 8 * (lane >> 5) + (i >> 2);
-  const int col = 32 * t + (lane & 16) + 4 * (i & 3);
-  const u32x2 lo = lds_read_tr(lds + lds_at<D>(row, col >> 3) + 2 * (col & 7));
-  const u32x2 hi = lds_read_tr(lds + lds_at<D>(row + 4, col >> 3) + 2 * (col & 7));
+// Operand with row or column lr and k = 16 s + 8 lh + (0..7) from 32 columns of a
+// row-major [k][column] tile in LDS; p: transposed_at of the lane plus 64 bytes a
+// column tile.
+template <class Tile>
+__device__ __forceinline__ u32x4 read_transposed(const char* p, int s) {
+  const u32x2 lo = lds_read_tr(p + s * Tile::at(16));
+  const u32x2 hi = lds_read_tr(p + s * Tile::at(16) + Tile::at(4));
   return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+template <class Tile, bool GROUPED>
+__device__ __forceinline__ int transposed_at() {
+  const int lane = threadIdx.x & 63, i = lane & 15;
+  return Tile::at(8 * (lane >> 5) + (i >> 2)) + 2 * (lane & 16) +
+         (GROUPED ? group_at(i & 3) : 8 * (i & 3));
 }
 
 // x as the sum of NT terms of the input type, each the rounding of what is left.
@@ -252,16 +283,25 @@ __device__ __forceinline__ int max_exponent(const u32x4 (&w)[N]) {
   return top ? exponent(Half::lo((uint32_t)top)) : kNone;
 }
 
+// Where a wave keeps its part of a segment's state in the workspace: the
+// accumulators as they are, 16 bytes a lane.
+template <int D>
+__device__ __forceinline__ int state_image(int wave, int dt, int quad, int lane) {
+  return (((wave * (D / 32) + dt) * 4 + quad) * 64 + lane) * 4;
+}
+
 // One segment of one head.  STATE_ONLY: forms the segment's own state (from
 // zero) into the workspace and no output.
 template <class T, int D, bool STATE_ONLY>
 __global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinParams p) {
   using L = LinShape<D>;
+  using Tile = typename L::Tile;
+  using Scores = typename L::Scores;
   constexpr int NT = kTerms<T>;
-  __shared__ __align__(16) char lds_q[STATE_ONLY ? 16 : L::TILEB];
-  __shared__ __align__(16) char lds_k[L::TILEB];
-  __shared__ __align__(16) char lds_v[L::TILEB];
-  __shared__ __align__(16) char lds_p[STATE_ONLY ? 16 : kChunk * 2 * kChunk];
+  __shared__ __align__(16) char lds_q[STATE_ONLY ? 16 : Tile::kBytes];
+  __shared__ __align__(16) char lds_k[Tile::kBytes];
+  __shared__ __align__(16) char lds_v[Tile::kBytes];
+  __shared__ __align__(16) char lds_p[STATE_ONLY ? 16 : Scores::kBytes];
   __shared__ __align__(16) float weight[kChunk];  // of row j in the state's update
 
   const int h = blockIdx.x % p.heads, slot = blockIdx.x / p.heads;
@@ -269,8 +309,7 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinPara
   const Segment sg = find_segment(p, slot);
   if (sg.b < 0) return;
   float* fin = fin_of(p, a, sg.b, h);
-  const bool last = sg.seg == sg.nseg - 1;
-  if (STATE_ONLY && last && !fin) return;
+  if (STATE_ONLY && sg.seg == sg.nseg - 1 && !fin) return;
   const int row0 = sg.seg * p.seglen;
   const int nrows = min(p.seglen, sg.len - row0);
 
@@ -280,39 +319,52 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinPara
   const int sh = a.reverse ? 1 : 0;
 
   const int batch = p.starts ? 0 : sg.b;
+  const int step = a.reverse ? -1 : 1;
+  // The token with the lowest address among rows c .. c + n - 1 of the segment.
+  auto lowest = [&](int c, int n) {
+    return (int64_t)(sg.start + (a.reverse ? sg.len - row0 - c - n : row0 + c));
+  };
   auto base_of = [&](const LinTensor& t) {
     return t.p + batch * t.s[0] + (h / t.div) * t.s[2];
   };
   const uint16_t* qp = base_of(a.q);
   const uint16_t* kp = base_of(a.k);
   const uint16_t* vp = base_of(a.v);
-  const int step = a.reverse ? -1 : 1;
-  auto token = [&](int r) { return sg.start + (a.reverse ? sg.len - 1 - row0 - r : row0 + r); };
+  Staged<D> sq, sk, sv;
+  auto load_chunk = [&](int c) {
+    const int n = min(kChunk, nrows - c);
+    const int64_t t = lowest(c, n);
+    if (!STATE_ONLY) load_rows<D>(sq, qp + t * a.q.s[1], a.q.s[1], step, n);
+    load_rows<D>(sk, kp + t * a.k.s[1], a.k.s[1], step, n);
+    load_rows<D>(sv, vp + t * a.v.s[1], a.v.s[1], step, n);
+  };
+  load_chunk(0);
 
   // State column 32 wave + lr, row 32 dt + 8 (i / 4) + 4 lh + i % 4.
   f32x16 S[L::DT];
   float* seg_state =
       p.ws + (((int64_t)blockIdx.y * p.nseg * (p.starts ? 1 : p.batch) + slot) * p.heads + h) * D * D;
   const int col = 32 * wave + lr;
-  {
-    const float* src = nullptr;
-    int ird = D, icd = 1;
-    if (!STATE_ONLY) {
-      if (p.segmented) {
-        src = seg_state;
-      } else {
-        src = init_of(p, a, sg.b, h);
-        ird = a.ird;
-        icd = a.icd;
-      }
+#pragma unroll
+  for (int dt = 0; dt < L::DT; ++dt) S[dt] = f32x16{};
+  if (!STATE_ONLY) {
+    if (p.segmented) {
+#pragma unroll
+      for (int dt = 0; dt < L::DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 x =
+              *reinterpret_cast<const f32x4*>(seg_state + state_image<D>(wave, dt, i, lane));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) S[dt][4 * i + j] = x[j];
+        }
+    } else if (const float* src = init_of(p, a, sg.b, h)) {
+#pragma unroll
+      for (int dt = 0; dt < L::DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          S[dt][i] = src[(32 * dt + 8 * (i / 4) + 4 * lh + i % 4) * a.ird + col * a.icd];
     }
-#pragma unroll
-    for (int dt = 0; dt < L::DT; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int d = 32 * dt + 8 * (i / 4) + 4 * lh + i % 4;
-        S[dt][i] = src ? src[d * ird + col * icd] : 0.f;
-      }
   }
 
   // P^T quadrants (32 keys j x 32 rows i) on and below the diagonal, dealt to the
@@ -336,14 +388,13 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinPara
   for (int t = 0; t < 2; ++t)
     rowf[t] = a.inter_scale * fast_exp2(g2 * (float)(32 * t + lr + 1 - sh));
 
-  Staged<D> sq, sk, sv;
-  {
-    const int n = min(kChunk, nrows);
-    if (!STATE_ONLY) load_rows<D>(sq, qp, a.q.s[1], token(0), step, n);
-    load_rows<D>(sk, kp, a.k.s[1], token(0), step, n);
-    load_rows<D>(sv, vp, a.v.s[1], token(0), step, n);
-  }
-  int weights_n = 0;  // rows of the chunk that `weight` is for
+  const int op_at = Tile::at(lr) + 16 * lh;  // operand reads of Q and K rows
+  const char* kt_p = lds_k + transposed_at<Tile, true>();
+  const char* vt_p = lds_v + transposed_at<Tile, false>() + 64 * wave;
+  const int p_at = Scores::at(lr);
+
+  int weights_n = 0;  // rows of the chunk that `weight` and dm1 (l^n - 1) are for
+  float dm1 = 0.f;
   int held = 0;       // S is held times 2^held (fp16)
   // |weight| < 2^weight_top (upd_scale 0 or not finite: no scaling to speak of)
   const int weight_top = min(max(exponent(a.upd_scale), -60), 60) + 1;
@@ -351,23 +402,19 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinPara
   for (int c = 0; c < nrows; c += kChunk) {
     const int n = min(kChunk, nrows - c);
     __syncthreads();  // the last chunk's LDS reads are done
-    if (!STATE_ONLY) store_rows<D>(sq, lds_q);
-    store_rows<D>(sk, lds_k);
-    store_rows<D>(sv, lds_v);
+    if (!STATE_ONLY) store_rows<D, true>(sq, lds_q);
+    store_rows<D, true>(sk, lds_k);
+    store_rows<D, false>(sv, lds_v);
     if (n != weights_n) {
       // Rows at or behind n are zeros: their weight only has to be finite.
       if (threadIdx.x < kChunk)
         weight[threadIdx.x] =
             a.upd_scale * fast_exp2(g2 * (float)max(n - 1 - (int)threadIdx.x + sh, 0));
       weights_n = n;
+      dm1 = expm1f(g * (float)n);
     }
     __syncthreads();
-    if (c + kChunk < nrows) {
-      const int m = min(kChunk, nrows - c - kChunk), t = token(c + kChunk);
-      if (!STATE_ONLY) load_rows<D>(sq, qp, a.q.s[1], t, step, m);
-      load_rows<D>(sk, kp, a.k.s[1], t, step, m);
-      load_rows<D>(sv, vp, a.v.s[1], t, step, m);
-    }
+    if (c + kChunk < nrows) load_chunk(c + kChunk);
 
     f32x16 o[2];
     if constexpr (!STATE_ONLY) {
@@ -377,18 +424,20 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinPara
         const int quad = wave + L::NW * nq;
         if (quad < 3) {
           const int it = quad > 0, jt = quad > 1;
+          const char* kq = lds_k + op_at + jt * Tile::at(32);
+          const char* qq = lds_q + op_at + it * Tile::at(32);
           f32x16 acc = {};
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            acc = T::mma32(ld16(lds_k + lds_at<D>(32 * jt + lr, 2 * kk + lh)),
-                           ld16(lds_q + lds_at<D>(32 * it + lr, 2 * kk + lh)), acc);
+            acc = T::mma32(ld16(kq + 32 * kk), ld16(qq + 32 * kk), acc);
+          char* pw = lds_p + p_at + it * Scores::at(32) + 64 * jt + 8 * lh;
 #pragma unroll
           for (int gi = 0; gi < 4; ++gi) {
             u32x2 w;
             w[0] = T::pack(acc[4 * gi] * pf[nq][4 * gi], acc[4 * gi + 1] * pf[nq][4 * gi + 1]);
             w[1] = T::pack(acc[4 * gi + 2] * pf[nq][4 * gi + 2],
                            acc[4 * gi + 3] * pf[nq][4 * gi + 3]);
-            st8(lds_p + lds_at<kChunk>(32 * it + lr, 4 * jt + gi) + 8 * lh, w);
+            st8(pw + 16 * gi, w);
           }
         }
       }
@@ -417,11 +466,9 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinPara
           for (int i = 0; i < 4; ++i)
             sf[i] = T::pack(S[dt][8 * half + 2 * i] * down, S[dt][8 * half + 2 * i + 1] * down);
 #pragma unroll
-          for (int it = 0; it < 2; ++it) {
-            const u32x2 x = ld8(lds_q + lds_at<D>(32 * it + lr, 4 * dt + 2 * half) + 8 * lh);
-            const u32x2 y = ld8(lds_q + lds_at<D>(32 * it + lr, 4 * dt + 2 * half + 1) + 8 * lh);
-            o[it] = T::mma32(sf, u32x4{x[0], x[1], y[0], y[1]}, o[it]);
-          }
+          for (int it = 0; it < 2; ++it)
+            o[it] = T::mma32(
+                sf, ld16(lds_q + op_at + it * Tile::at(32) + 64 * dt + 32 * half), o[it]);
         }
 #pragma unroll
       for (int it = 0; it < 2; ++it)
@@ -433,16 +480,13 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinPara
     // S = l^n S + K^T (weight V), and O^T += V^T P^T on the way.  The decay as
     // S + S (l^n - 1): the factor's own rounding, which a slow decay would
     // compound over hundreds of chunks, is then relative to the small difference.
-    {
-      const float dm1 = expm1f(g * (float)n);
 #pragma unroll
-      for (int dt = 0; dt < L::DT; ++dt)
+    for (int dt = 0; dt < L::DT; ++dt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) S[dt][i] = fmaf(S[dt][i], dm1, S[dt][i]);
-    }
+      for (int i = 0; i < 16; ++i) S[dt][i] = fmaf(S[dt][i], dm1, S[dt][i]);
     u32x4 vts[kChunk / 16];
 #pragma unroll
-    for (int s = 0; s < kChunk / 16; ++s) vts[s] = read_transposed<D>(lds_v, s, wave);
+    for (int s = 0; s < kChunk / 16; ++s) vts[s] = read_transposed<Tile>(vt_p, s);
     if constexpr (T::kId == 0) {
       const int e = max_exponent(vts);
       const int want = 13 - e - weight_top;
@@ -463,58 +507,75 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinPara
       if constexpr (!STATE_ONLY) {
 #pragma unroll
         for (int it = s / 2; it < 2; ++it)
-          o[it] = T::mma32(vt, ld16(lds_p + lds_at<kChunk>(32 * it + lr, 2 * s + lh)), o[it]);
+          o[it] = T::mma32(vt, ld16(lds_p + p_at + it * Scores::at(32) + 32 * s + 16 * lh), o[it]);
       }
       float x[8];
+      const f32x4 w0 = *reinterpret_cast<const f32x4*>(weight + 16 * s + 8 * lh) * hold;
+      const f32x4 w1 = *reinterpret_cast<const f32x4*>(weight + 16 * s + 8 * lh + 4) * hold;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[2 * i] = T::lo(vt[i]) * (weight[16 * s + 8 * lh + 2 * i] * hold);
-        x[2 * i + 1] = T::hi(vt[i]) * (weight[16 * s + 8 * lh + 2 * i + 1] * hold);
+        x[2 * i] = T::lo(vt[i]) * (i < 2 ? w0[2 * i] : w1[2 * i - 4]);
+        x[2 * i + 1] = T::hi(vt[i]) * (i < 2 ? w0[2 * i + 1] : w1[2 * i - 3]);
       }
       u32x4 term[NT];
       split_terms<T, NT>(x, term);
 #pragma unroll
       for (int dt = 0; dt < L::DT; ++dt) {
-        const u32x4 kt = read_transposed<D>(lds_k, s, dt);
+        const u32x4 kt = read_transposed<Tile>(kt_p + 64 * dt, s);
 #pragma unroll
         for (int t = 0; t < NT; ++t) S[dt] = T::mma32(kt, term[t], S[dt]);
       }
     }
 
     if constexpr (!STATE_ONLY) {
+      const int64_t at = batch * a.os[0] + lowest(c, n) * a.os[1] + h * a.os[2];
+      const uint32_t size = a.out_f32 ? 4 : 2, row = size * (uint32_t)a.os[1];
+      const rsrc_t rs = make_rsrc(static_cast<char*>(a.out) + at * size,
+                                  (uint32_t)((n - 1) * a.os[1] + D) * size);
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
         const int r = 32 * it + lr;
-        if (r >= n) continue;
-        const int64_t at = batch * a.os[0] + token(c + r) * a.os[1] + h * a.os[2] + 32 * wave + 4 * lh;
+        const uint32_t off = (uint32_t)(step > 0 ? r : n - 1 - r) * row + size * (32 * wave + 4 * lh);
         if (a.out_f32) {
-          float* out = static_cast<float*>(a.out) + at;
 #pragma unroll
           for (int gi = 0; gi < 4; ++gi)
-            *reinterpret_cast<f32x4*>(out + 8 * gi) =
-                f32x4{o[it][4 * gi], o[it][4 * gi + 1], o[it][4 * gi + 2], o[it][4 * gi + 3]};
+            __builtin_amdgcn_raw_buffer_store_b128(
+                __builtin_bit_cast(u32x4, f32x4{o[it][4 * gi], o[it][4 * gi + 1], o[it][4 * gi + 2],
+                                                o[it][4 * gi + 3]}),
+                rs, r < n ? off + 32 * gi : 0xffffffffu, 0, 0);
         } else {
-          uint16_t* out = static_cast<uint16_t*>(a.out) + at;
 #pragma unroll
           for (int gi = 0; gi < 4; ++gi)
-            st8(out + 8 * gi, u32x2{T::pack(o[it][4 * gi], o[it][4 * gi + 1]),
-                                    T::pack(o[it][4 * gi + 2], o[it][4 * gi + 3])});
+            __builtin_amdgcn_raw_buffer_store_b64(
+                u32x2{T::pack(o[it][4 * gi], o[it][4 * gi + 1]),
+                      T::pack(o[it][4 * gi + 2], o[it][4 * gi + 3])},
+                rs, r < n ? off + 16 * gi : 0xffffffffu, 0, 0);
         }
       }
     }
   }
 
-  float* dst = STATE_ONLY ? seg_state : (p.segmented ? nullptr : fin);
-  if (!dst) return;
+  const float out = pow2(-held);
+  if (STATE_ONLY) {
 #pragma unroll
-  for (int dt = 0; dt < L::DT; ++dt)
+    for (int dt = 0; dt < L::DT; ++dt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      dst[(32 * dt + 8 * (i / 4) + 4 * lh + i % 4) * D + col] = S[dt][i] * pow2(-held);
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(seg_state + state_image<D>(wave, dt, i, lane)) =
+            f32x4{S[dt][4 * i] * out, S[dt][4 * i + 1] * out, S[dt][4 * i + 2] * out,
+                  S[dt][4 * i + 3] * out};
+  } else if (!p.segmented && fin) {
+#pragma unroll
+    for (int dt = 0; dt < L::DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        fin[(32 * dt + 8 * (i / 4) + 4 * lh + i % 4) * D + col] = S[dt][i] * out;
+  }
 }
 
 // Joins the segments' states in order: each slot's own state becomes the state
-// before it, and the last sum the final state.  A thread holds four components.
+// before it, and the last sum the final state.  A thread holds four components, in
+// the workspace's layout (state_image): rows d .. d + 3 of column e.
 template <int D>
 __global__ __launch_bounds__(256) void linear_scan_kernel(LinParams p) {
   constexpr int PARTS = D * D / 1024;
@@ -524,8 +585,7 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinParams p) {
   int first = b * p.nseg, len = p.seqlen;
   if (p.starts) {
     int start, n = 0;
-    const int lane = threadIdx.x & 63;
-    for (int i = lane; i < b; i += 64) {
+    for (int i = threadIdx.x & 63; i < b; i += 64) {
       packed_rows(p, i, start, len);
       n += (len + p.seglen - 1) / p.seglen;
     }
@@ -543,10 +603,11 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinParams p) {
   const float g = decay_of(p, h);
   const float dm1 = expm1f(g * (float)p.seglen);
   f32x4 S = {0.f, 0.f, 0.f, 0.f};
+  const int lane = at / 4 % 64, quad = at / 256 % 4, dt = at / 1024 % (D / 32);
+  const int d = 32 * dt + 8 * quad + 4 * (lane >> 5), e = 32 * (at / (32 * D)) + (lane & 31);
   if (init) {
-    const int d = at / D, e = at % D;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) S[i] = init[d * a.ird + (e + i) * a.icd];
+    for (int i = 0; i < 4; ++i) S[i] = init[(d + i) * a.ird + e * a.icd];
   }
   for (int s = 0; s < nseg; ++s, state += next) {
     f32x4 u = {0.f, 0.f, 0.f, 0.f};
@@ -556,7 +617,10 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinParams p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) S[i] = fmaf(S[i], f, S[i]) + u[i];
   }
-  if (fin) *reinterpret_cast<f32x4*>(fin + at) = S;
+  if (fin) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fin[(d + i) * D + e] = S[i];
+  }
 }
 
 // Gradients of shared heads: the fp32 parts of a KV head's query heads, in order.
@@ -677,14 +741,14 @@ size_t state_bytes(const LinParams& p, int64_t slots, int D) {
 
 template <class T, int D>
 hipError_t launch_passes(LinParams& p, int64_t slots, hipStream_t st) {
-  using L = LinShape<D>;
-  const dim3 grid((unsigned)(slots * p.heads), p.npass);
+  const dim3 grid((unsigned)(slots * p.heads), p.npass), block(LinShape<D>::THREADS);
   if (p.segmented) {
-    hipLaunchKernelGGL((linear_kernel<T, D, true>), grid, dim3(L::THREADS), 0, st, p);
-    hipLaunchKernelGGL((linear_scan_kernel<D>), dim3((unsigned)(D * D / 1024 * p.batch * p.heads), p.npass),
-                       dim3(256), 0, st, p);
+    hipLaunchKernelGGL((linear_kernel<T, D, true>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((linear_scan_kernel<D>),
+                       dim3((unsigned)(D * D / 1024 * p.batch * p.heads), p.npass), dim3(256), 0,
+                       st, p);
   }
-  hipLaunchKernelGGL((linear_kernel<T, D, false>), grid, dim3(L::THREADS), 0, st, p);
+  hipLaunchKernelGGL((linear_kernel<T, D, false>), grid, block, 0, st, p);
   return hipGetLastError();
 }
 

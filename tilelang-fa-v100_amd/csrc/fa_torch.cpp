@@ -586,6 +586,8 @@ PyObject* linear_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !linear_common(a, a[7], a[8], prefix->size(0), c, q, &p, &state))
       return none();
     const at::Tensor &k = THPVariable_Unpack(a[1]), &v = THPVariable_Unpack(a[2]);
+    const int64_t lim = int64_t(1) << 24;
+    if (q->stride(0) >= lim || k.stride(0) >= lim || v.stride(0) >= lim) return none();
     at::Tensor out;
     int status;
     {

@@ -87,6 +87,12 @@ def _require_place(named):
     require_same(named, "device")
 
 
+def _rows(t):
+    """rows_ready, and a copy where the sequence stride is 2^24 elements or more."""
+    t = rows_ready(t)
+    return t if t.stride(-3) < 1 << 24 or t.shape[-3] == 1 else t.contiguous()
+
+
 def _scale(scale, D):
     return float(scale) if scale is not None else D ** -0.5
 
@@ -134,7 +140,7 @@ def _forward(q, k, v, log_decay, scale, initial_state, want_final):
                 torch.zeros((B, H, D, D), dtype=torch.float32, device=q.device)
         return out, final
     final = torch.empty((B, H, D, D), dtype=torch.float32, device=q.device) if want_final else None
-    q, k, v, log_decay = rows_ready(q), rows_ready(k), rows_ready(v), log_decay.contiguous()
+    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     a = _lib.LinearArgs()
     _set_qkv(a, q, k, v, log_decay, scale)
     a.out = out.data_ptr()
@@ -162,7 +168,7 @@ def _backward(q, k, v, dout, log_decay, scale, initial_state, d_final, want_d_in
         return dq, dk, dv, d_initial
     d_initial = torch.empty((B, H, D, D), dtype=torch.float32, device=q.device) \
         if want_d_initial else None
-    q, k, v, dout = rows_ready(q), rows_ready(k), rows_ready(v), rows_ready(dout)
+    q, k, v, dout = _rows(q), _rows(k), _rows(v), _rows(dout)
     log_decay = log_decay.contiguous()
     a = _lib.LinearBwdArgs()
     _set_qkv(a, q, k, v, log_decay, scale)
@@ -304,8 +310,8 @@ def linear_attn_prefill(q, k, v, log_decay, state, query_start_loc, prefix_kv_le
         raise ValueError("out must match q in shape, dtype and device")
     if B == 0 or q.shape[0] == 0:
         return out
-    q, k, v, log_decay = rows_ready(q), rows_ready(k), rows_ready(v), log_decay.contiguous()
-    target = rows_ready(out)
+    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
+    target = _rows(out)
     starts = as_int32(query_start_loc, q.device, "query_start_loc")
     prefix = as_int32(prefix_kv_lens, q.device, "prefix_kv_lens")
     slots = as_int32(state_indices, q.device, "state_indices") \
