@@ -16,11 +16,11 @@
 // One kernel runs all of them ("passes"), in one launch.
 //
 // Work split: a workgroup holds one (sequence, head, segment)'s state in
-// registers and walks its chunks; each wave owns 32 of the state's columns (D / 32
-// waves).  Where sequences x heads are too few for the GPU, sequences are cut
-// into segments: one launch forms every segment's own state, one joins them in
-// order (linear_scan_kernel), and the main launch starts each segment from its
-// joined state.
+// registers and walks its chunks; each wave owns 16 of the state's columns (D / 16
+// waves, 128 registers each: at head_dim 128 two workgroups and 16 waves on a CU).  Where sequences x heads are too few for the GPU, sequences are cut
+// into segments: one launch forms every segment's own state, and the main launch
+// starts each segment from the states of those before it, which it adds up itself
+// (few segments) or finds joined by linear_scan_kernel.
 //
 // Registers and LDS: the state's accumulators (row d in the registers, column e
 // in the lane) are, rounded, the A operand of O^T = S^T Q^T as they stand: S never
@@ -76,8 +76,16 @@ struct LinParams {
   int32_t nseg;    // dense: segments of a sequence; packed: slots in all
   int32_t seglen;  // rows of a segment, a multiple of kChunk
   int32_t nstates;
-  int32_t segmented;
+  int32_t join;
 };
+
+// How a segment comes by the state before it: there is one segment; from the
+// states of those before it, which the main kernel adds up; or linear_scan_kernel
+// has put it into its slot.
+enum { kWhole = 0, kAdded = 1, kScanned = 2 };
+// Segments of a sequence that are added up (none at head_dim 256, whose kernel has
+// no registers for it).
+constexpr int max_added(int D) { return D < 256 ? 8 : 1; }
 
 struct Segment {
   int b, seg, nseg;  // sequence, segment, segments of the sequence; b < 0: none
@@ -155,86 +163,96 @@ __device__ __forceinline__ float decay_of(const LinParams& p, int h) {
   return g < -1e30f ? -1e30f : g;
 }
 
-// LDS rows of `W` 16-bit elements.  Rows are 64 bytes (16 banks) apart in bank
-// terms and every fourth row 16 bytes further, so that the operand reads (16 bytes
-// of 16 rows) and the transposing reads (64 bytes of 4 rows) each touch every bank
-// once, with addresses that are one lane register plus an immediate: with an XOR
-// swizzle instead the compiler held some 40 address registers and spilled.
+// LDS rows of `W` 16-bit elements, 32 bytes (8 banks) further apart than they are
+// long: the operand reads (16 bytes of 16 rows) and the transposing reads (32 bytes
+// of 16 rows) then have no bank conflicts (3.9 and 2.6 cycles a wave; 6.4 and 3.8 at
+// 16 or 64 bytes), and every address is one lane register plus an immediate (an XOR
+// swizzle took some 40 address registers).
 template <int W>
 struct Rows16 {
-  static constexpr int kStride = 2 * W + 64;
-  static constexpr int kBytes = kChunk * kStride + kChunk / 4 * 16;
-  __device__ static __forceinline__ int at(int r) { return r * kStride + (r >> 2) * 16; }
+  static constexpr int kStride = 2 * W + 32;
+  static constexpr int kBytes = kChunk * kStride;
+  __device__ static __forceinline__ int at(int r) { return r * kStride; }
 };
 
 template <int D>
 struct LinShape {
-  static constexpr int NW = D / 32;        // waves
+  static constexpr int NW = D / 16;        // waves
   static constexpr int THREADS = 64 * NW;
   static constexpr int CPR = D / 8;        // 16-byte chunks of a row
-  static constexpr int DT = D / 32;        // 32-row tiles of the state
+  static constexpr int RPT = THREADS / CPR;  // rows the workgroup moves at a time: 32
+  static constexpr int DT = D / 16;        // 16-row tiles of the state
   using Tile = Rows16<D>;
   using Scores = Rows16<kChunk>;
 };
 
-// Q and K rows are kept with their 4-element groups in the order 0, 2, 1, 3 of
-// each 16: lane half lh then finds the 8 components that the state's accumulators
-// give it (4 lh + 0..3 and 8 + 4 lh + 0..3) in one 16-byte read.
-__device__ __forceinline__ int group_at(int g) { return 8 * ((g & 1) * 2 + (g >> 1)); }
+// Q's rows and P's are kept with their 4-element groups of each 32 in the order 0,
+// 4, 1, 5, 2, 6, 3, 7.  A lane quarter l then finds in one 16-byte read the 8
+// components (keys) that it has in the other operand: 4 l + 0..3 and 16 + 4 l + 0..3,
+// from two of the state's 16-row tiles or two transposing reads of V.  Byte offset
+// of group g of a row:
+__device__ __forceinline__ int group_at(int g) {
+  return 64 * (g >> 3) + 16 * (g & 3) + 8 * ((g >> 2) & 1);
+}
 
-// A chunk's rows of one tensor on the way to LDS, 16 bytes x 4 a thread: row
-// 16 u + tid / CPR.  Rows at or behind n are zeros.
-template <int D>
+// A chunk's rows of one tensor on the way to LDS, 16 bytes x 2 a thread: row
+// 32 u + tid / CPR.  Rows at or behind n are zeros.
 struct Staged {
-  u32x4 x[4];
+  u32x4 x[2];
 };
-// `lowest`: the chunk's row with the lowest address; rows go up from it (step 1)
-// or down to it from row 0 (step -1).
+// Byte offset of row r of a chunk of n rows from its lowest address: rows go up
+// from it (step 1) or down to it (step -1); out of any range behind n.
+__device__ __forceinline__ uint32_t row_offset(int r, int n, int step, uint32_t row, uint32_t at) {
+  return r < n ? (uint32_t)(step > 0 ? r : n - 1 - r) * row + at : 0xffffffffu;
+}
 template <int D>
-__device__ __forceinline__ void load_rows(Staged<D>& s, const uint16_t* lowest, int64_t stride,
-                                          int step, int n) {
+__device__ __forceinline__ void load_rows(Staged& s, const uint16_t* lowest, int64_t stride,
+                                          int step, int n, int tid) {
   using L = LinShape<D>;
   const rsrc_t rs = make_rsrc(lowest, (uint32_t)((n - 1) * stride + D) * 2u);
-  const int r0 = (int)threadIdx.x / L::CPR;
-  const uint32_t row = 2 * (uint32_t)stride;  // bytes
-  const uint32_t at = 16 * (threadIdx.x % L::CPR);
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int r = 16 * u + r0;
-    const uint32_t off = (uint32_t)(step > 0 ? r : n - 1 - r) * row + at;
-    s.x[u] = __builtin_amdgcn_raw_buffer_load_b128(rs, r < n ? off : 0xffffffffu, 0, 0);
+  for (int u = 0; u < 2; ++u)
+    s.x[u] = __builtin_amdgcn_raw_buffer_load_b128(
+        rs,
+        row_offset(L::RPT * u + tid / L::CPR, n, step, 2 * (uint32_t)stride, 16 * (tid % L::CPR)),
+        0, 0);
+}
+// Where a thread's 16 bytes of row tid / CPR stand in LDS.
+template <int D>
+__device__ __forceinline__ int place_of(int tid) {
+  using L = LinShape<D>;
+  return L::Tile::at(tid / L::CPR) + 16 * (tid % L::CPR);
+}
+template <int D>
+__device__ __forceinline__ void store_grouped(const Staged& s, char* lds, int tid) {
+  using L = LinShape<D>;
+  char* p = lds + L::Tile::at(tid / L::CPR) + group_at(2 * (tid % L::CPR));
+#pragma unroll
+  for (int u = 0; u < 2; ++u, p += L::Tile::at(L::RPT)) {
+    st8(p, u32x2{s.x[u][0], s.x[u][1]});
+    st8(p + 16, u32x2{s.x[u][2], s.x[u][3]});
   }
 }
-template <int D, bool GROUPED>
-__device__ __forceinline__ void store_rows(const Staged<D>& s, char* lds) {
+template <int D>
+__device__ __forceinline__ void store_rows(const Staged& s, char* lds, int tid) {
   using L = LinShape<D>;
-  const int r0 = (int)threadIdx.x / L::CPR, c = threadIdx.x % L::CPR;
-  char* p = lds + L::Tile::at(r0) + (GROUPED ? 32 * (c >> 1) + 8 * (c & 1) : 16 * c);
 #pragma unroll
-  for (int u = 0; u < 4; ++u, p += L::Tile::at(16)) {
-    if constexpr (GROUPED) {
-      st8(p, u32x2{s.x[u][0], s.x[u][1]});
-      st8(p + 16, u32x2{s.x[u][2], s.x[u][3]});
-    } else {
-      st16(p, s.x[u]);
-    }
-  }
+  for (int u = 0; u < 2; ++u) st16(lds + place_of<D>(tid) + u * L::Tile::at(L::RPT), s.x[u]);
 }
 
-// Operand with row or column lr and k = 16 s + 8 lh + (0..7) from 32 columns of a
-// row-major [k][column] tile in LDS; p: transposed_at of the lane plus 64 bytes a
-// column tile.
+// Operand with row or column lane % 16 and k = 32 s + 4 (lane / 16) + 0..3 and the
+// same + 16, from 16 columns of a row-major [k][column] tile in LDS; p: the tile, transposed_at of the
+// lane, and the 16 columns' place.
 template <class Tile>
 __device__ __forceinline__ u32x4 read_transposed(const char* p, int s) {
-  const u32x2 lo = lds_read_tr(p + s * Tile::at(16));
-  const u32x2 hi = lds_read_tr(p + s * Tile::at(16) + Tile::at(4));
+  const u32x2 lo = lds_read_tr(p + s * Tile::at(32));
+  const u32x2 hi = lds_read_tr(p + s * Tile::at(32) + Tile::at(16));
   return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
-template <class Tile, bool GROUPED>
+template <class Tile>
 __device__ __forceinline__ int transposed_at() {
-  const int lane = threadIdx.x & 63, i = lane & 15;
-  return Tile::at(8 * (lane >> 5) + (i >> 2)) + 2 * (lane & 16) +
-         (GROUPED ? group_at(i & 3) : 8 * (i & 3));
+  const int lane = threadIdx.x & 63;
+  return Tile::at(4 * (lane >> 4) + ((lane & 15) >> 2)) + 8 * (lane & 3);
 }
 
 // x as the sum of NT terms of the input type, each the rounding of what is left.
@@ -286,35 +304,37 @@ __device__ __forceinline__ int max_exponent(const u32x4 (&w)[N]) {
 // Where a wave keeps its part of a segment's state in the workspace: the
 // accumulators as they are, 16 bytes a lane.
 template <int D>
-__device__ __forceinline__ int state_image(int wave, int dt, int quad, int lane) {
-  return (((wave * (D / 32) + dt) * 4 + quad) * 64 + lane) * 4;
+__device__ __forceinline__ int state_image(int wave, int dt, int lane) {
+  return ((wave * (D / 16) + dt) * 64 + lane) * 4;
 }
 
 // One segment of one head.  STATE_ONLY: forms the segment's own state (from
 // zero) into the workspace and no output.
 template <class T, int D, bool STATE_ONLY>
-__global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinParams p) {
+__global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear_kernel(LinParams p) {
   using L = LinShape<D>;
   using Tile = typename L::Tile;
   using Scores = typename L::Scores;
   constexpr int NT = kTerms<T>;
+  // Whether 128 or more registers hold what a chunk does not change.
+  constexpr bool kKeep = D < 256;
   __shared__ __align__(16) char lds_q[STATE_ONLY ? 16 : Tile::kBytes];
   __shared__ __align__(16) char lds_k[Tile::kBytes];
   __shared__ __align__(16) char lds_v[Tile::kBytes];
   __shared__ __align__(16) char lds_p[STATE_ONLY ? 16 : Scores::kBytes];
   __shared__ __align__(16) float weight[kChunk];  // of row j in the state's update
+  __shared__ float powers[STATE_ONLY ? 1 : kChunk + 17];
 
   const int h = blockIdx.x % p.heads, slot = blockIdx.x / p.heads;
   const LinPass& a = p.pass[blockIdx.y];
   const Segment sg = find_segment(p, slot);
   if (sg.b < 0) return;
-  float* fin = fin_of(p, a, sg.b, h);
-  if (STATE_ONLY && sg.seg == sg.nseg - 1 && !fin) return;
+  if (STATE_ONLY && sg.seg == sg.nseg - 1) return;  // no segment starts from it
   const int row0 = sg.seg * p.seglen;
   const int nrows = min(p.seglen, sg.len - row0);
 
   const int lane = threadIdx.x & 63, wave = wave_id();
-  const int lr = lane & 31, lh = lane >> 5;
+  const int lc = lane & 15, lq = lane >> 4;
   const float g = decay_of(p, h), g2 = g * kLog2e;
   const int sh = a.reverse ? 1 : 0;
 
@@ -330,81 +350,131 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinPara
   const uint16_t* qp = base_of(a.q);
   const uint16_t* kp = base_of(a.k);
   const uint16_t* vp = base_of(a.v);
-  Staged<D> sq, sk, sv;
-  auto load_chunk = [&](int c) {
+  Staged sq, sk, sv;
+  auto load_chunk = [&](int c, int tid) {
     const int n = min(kChunk, nrows - c);
     const int64_t t = lowest(c, n);
-    if (!STATE_ONLY) load_rows<D>(sq, qp + t * a.q.s[1], a.q.s[1], step, n);
-    load_rows<D>(sk, kp + t * a.k.s[1], a.k.s[1], step, n);
-    load_rows<D>(sv, vp + t * a.v.s[1], a.v.s[1], step, n);
+    if (!STATE_ONLY) load_rows<D>(sq, qp + t * a.q.s[1], a.q.s[1], step, n, tid);
+    load_rows<D>(sk, kp + t * a.k.s[1], a.k.s[1], step, n, tid);
+    load_rows<D>(sv, vp + t * a.v.s[1], a.v.s[1], step, n, tid);
   };
-  load_chunk(0);
+  load_chunk(0, threadIdx.x);
 
-  // State column 32 wave + lr, row 32 dt + 8 (i / 4) + 4 lh + i % 4.
-  f32x16 S[L::DT];
+  // State column 16 wave + lc, rows 16 dt + 4 lq + (0..3).
+  f32x4 S[L::DT];
   float* seg_state =
       p.ws + (((int64_t)blockIdx.y * p.nseg * (p.starts ? 1 : p.batch) + slot) * p.heads + h) * D * D;
-  const int col = 32 * wave + lr;
+  const int col = 16 * wave + lc;
 #pragma unroll
-  for (int dt = 0; dt < L::DT; ++dt) S[dt] = f32x16{};
+  for (int dt = 0; dt < L::DT; ++dt) S[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (!STATE_ONLY) {
-    if (p.segmented) {
+    if (p.join == kScanned) {
 #pragma unroll
       for (int dt = 0; dt < L::DT; ++dt)
+        S[dt] = *reinterpret_cast<const f32x4*>(seg_state + state_image<D>(wave, dt, lane));
+    } else {
+      if (const float* src = init_of(p, a, sg.b, h)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 x =
-              *reinterpret_cast<const f32x4*>(seg_state + state_image<D>(wave, dt, i, lane));
+        for (int dt = 0; dt < L::DT; ++dt)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) S[dt][4 * i + j] = x[j];
-        }
-    } else if (const float* src = init_of(p, a, sg.b, h)) {
+          for (int i = 0; i < 4; ++i)
+            S[dt][i] = src[(16 * dt + 4 * lq + i) * a.ird + col * a.icd];
+      }
+      // The states of the segments before, in order.
+      if constexpr (kKeep) {
+      const float decay = expm1f(g * (float)p.seglen);
+      const int64_t next = (int64_t)p.heads * D * D;
+      for (int s = sg.seg; s > 0; --s) {
+        const float* u = seg_state - s * next + state_image<D>(wave, 0, lane);
+        f32x4 x[L::DT];
 #pragma unroll
-      for (int dt = 0; dt < L::DT; ++dt)
+        for (int dt = 0; dt < L::DT; ++dt) x[dt] = *reinterpret_cast<const f32x4*>(u + 256 * dt);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          S[dt][i] = src[(32 * dt + 8 * (i / 4) + 4 * lh + i % 4) * a.ird + col * a.icd];
-    }
-  }
-
-  // P^T quadrants (32 keys j x 32 rows i) on and below the diagonal, dealt to the
-  // waves: 0 is (0, 0), 1 is (row tile 1, key tile 0), 2 is (1, 1).
-  constexpr int NQ = L::NW == 2 ? 2 : 1;
-  float pf[NQ][16];
-  if (!STATE_ONLY) {
+        for (int dt = 0; dt < L::DT; ++dt)
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const int quad = wave + L::NW * n;
-      const int row = 32 * (quad > 0) + lr;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = 32 * (quad > 1) + 8 * (i / 4) + 4 * lh + i % 4;
-        pf[n][i] = key <= row ? a.p_scale * fast_exp2(g2 * (float)(row - key)) : 0.f;
+          for (int i = 0; i < 4; ++i) S[dt][i] = fmaf(S[dt][i], decay, S[dt][i]) + x[dt][i];
+      }
       }
     }
   }
-  float rowf[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-    rowf[t] = a.inter_scale * fast_exp2(g2 * (float)(32 * t + lr + 1 - sh));
 
-  const int op_at = Tile::at(lr) + 16 * lh;  // operand reads of Q and K rows
-  const char* kt_p = lds_k + transposed_at<Tile, true>();
-  const char* vt_p = lds_v + transposed_at<Tile, false>() + 64 * wave;
-  const int p_at = Scores::at(lr);
+  // P^T tiles (16 keys j x 16 rows i) on and below the diagonal, dealt to the waves
+  // in the order (row tile, key tile) = (0, 0), (1, 0), (1, 1), (2, 0), ...
+  constexpr int NP = (10 + L::NW - 1) / L::NW;
+  static_assert(L::THREADS >= kChunk + 17, "a thread for each power");
+  // l^e for e = 0..64, and 0 for e = -16..-1 (keys behind their row).  At head_dim
+  // 256 the factors of P and of O's rows are read from it where they are used: a
+  // wave's 128 registers have no room for them.
+  const float* power = powers + 16;
+  if (!STATE_ONLY && threadIdx.x < kChunk + 17) {
+    const int e = (int)threadIdx.x - 16;
+    powers[threadIdx.x] = e < 0 ? 0.f : fast_exp2(g2 * (float)e);
+  }
+
+  const int op_at = Tile::at(lc) + 16 * lq;  // operand reads of Q and K rows
+  const char* kt_p = lds_k + transposed_at<Tile>();
+  const char* vt_p = lds_v + transposed_at<Tile>() + 32 * wave;
+  const int p_at = Scores::at(lc);
+
+  // The two tiles above the diagonal that O's 32-key steps take in.
+  if (!STATE_ONLY && threadIdx.x < 64) {
+    const int t = threadIdx.x >> 5, r = (threadIdx.x & 31) >> 1;
+    for (int g = 0; g < 2; ++g)
+      st8(lds_p + Scores::at(32 * t + r) + group_at(4 * (2 * t + 1) + 2 * (threadIdx.x & 1) + g),
+          u32x2{0, 0});
+  }
 
   int weights_n = 0;  // rows of the chunk that `weight` and dm1 (l^n - 1) are for
   float dm1 = 0.f;
   int held = 0;       // S is held times 2^held (fp16)
+  const float p_scale = a.p_scale, inter_scale = a.inter_scale;
+  auto p_factor = [&](int tile, int i) {
+    const int it = (tile >= 1) + (tile >= 3) + (tile >= 6), jt = tile - it * (it + 1) / 2;
+    return p_scale * power[16 * (it - jt) + lc - 4 * lq - i];  // row - key of acc[i]
+  };
+  auto row_factor = [&](int it) { return power[16 * it + lc + 1 - sh]; };
+  float pf[NP][4], rowf[4];
+  if constexpr (!STATE_ONLY && kKeep) {
+    __syncthreads();
+#pragma unroll
+    for (int np = 0; np < NP; ++np)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pf[np][i] = p_factor(min(wave + L::NW * np, 9), i);
+#pragma unroll
+    for (int it = 0; it < 4; ++it) rowf[it] = row_factor(it);
+  }
   // |weight| < 2^weight_top (upd_scale 0 or not finite: no scaling to speak of)
   const int weight_top = min(max(exponent(a.upd_scale), -60), 60) + 1;
 
+  // The rows of O that the last chunk left in V's place, 16 bytes x 2 a thread (at
+  // the places where the thread puts its part of the next V).
+  auto write_rows = [&](int c, int n, int tid) {
+    const rsrc_t rs = make_rsrc(static_cast<uint16_t*>(a.out) + batch * a.os[0] +
+                                    lowest(c, n) * a.os[1] + h * a.os[2],
+                                (uint32_t)((n - 1) * a.os[1] + D) * 2u);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      __builtin_amdgcn_raw_buffer_store_b128(
+          ld16(lds_v + place_of<D>(tid) + u * Tile::at(L::RPT)), rs,
+          row_offset(L::RPT * u + tid / L::CPR, n, step, 2 * (uint32_t)a.os[1],
+                     16 * (tid % L::CPR)),
+          0, 0);
+  };
+
   for (int c = 0; c < nrows; c += kChunk) {
     const int n = min(kChunk, nrows - c);
-    __syncthreads();  // the last chunk's LDS reads are done
-    if (!STATE_ONLY) store_rows<D, true>(sq, lds_q);
-    store_rows<D, true>(sk, lds_k);
-    store_rows<D, false>(sv, lds_v);
+    // At head_dim 256 addresses are formed anew in every chunk: kept, they are the
+    // registers that no longer fit, and a reload from scratch waits for the rows on
+    // their way.
+    int tid = threadIdx.x;
+    if constexpr (!kKeep) asm volatile("" : "+v"(tid));
+    __syncthreads();  // the last chunk's LDS reads are done, and its O is there
+    if constexpr (!STATE_ONLY) {
+      if (c > 0 && !a.out_f32) write_rows(c - kChunk, kChunk, tid);
+      store_grouped<D>(sq, lds_q, tid);
+    }
+    store_rows<D>(sk, lds_k, tid);
+    store_rows<D>(sv, lds_v, tid);
     if (n != weights_n) {
       // Rows at or behind n are zeros: their weight only has to be finite.
       if (threadIdx.x < kChunk)
@@ -414,144 +484,141 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinPara
       dm1 = expm1f(g * (float)n);
     }
     __syncthreads();
-    if (c + kChunk < nrows) load_chunk(c + kChunk);
+    if (c + kChunk < nrows) load_chunk(c + kChunk, tid);
 
-    f32x16 o[2];
+    u32x4 vt[kChunk / 32];  // the wave's columns of V, for O and for the update
+#pragma unroll
+    for (int s = 0; s < kChunk / 32; ++s) vt[s] = read_transposed<Tile>(vt_p, s);
+    f32x4 o[4];
     if constexpr (!STATE_ONLY) {
       // P^T = K Q^T with the decay, rounded, as P's rows in LDS.
 #pragma unroll
-      for (int nq = 0; nq < NQ; ++nq) {
-        const int quad = wave + L::NW * nq;
-        if (quad < 3) {
-          const int it = quad > 0, jt = quad > 1;
-          const char* kq = lds_k + op_at + jt * Tile::at(32);
-          const char* qq = lds_q + op_at + it * Tile::at(32);
-          f32x16 acc = {};
+      for (int np = 0; np < NP; ++np) {
+        const int tile = wave + L::NW * np;
+        if (tile < 10) {
+          const int it = (tile >= 1) + (tile >= 3) + (tile >= 6), jt = tile - it * (it + 1) / 2;
+          const char* kq = lds_k + Tile::at(16 * jt + lc) + 8 * lq;
+          const char* qq = lds_q + op_at + it * Tile::at(16);
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            acc = T::mma32(ld16(kq + 32 * kk), ld16(qq + 32 * kk), acc);
-          char* pw = lds_p + p_at + it * Scores::at(32) + 64 * jt + 8 * lh;
-#pragma unroll
-          for (int gi = 0; gi < 4; ++gi) {
-            u32x2 w;
-            w[0] = T::pack(acc[4 * gi] * pf[nq][4 * gi], acc[4 * gi + 1] * pf[nq][4 * gi + 1]);
-            w[1] = T::pack(acc[4 * gi + 2] * pf[nq][4 * gi + 2],
-                           acc[4 * gi + 3] * pf[nq][4 * gi + 3]);
-            st8(pw + 16 * gi, w);
+          for (int kk = 0; kk < D / 32; ++kk) {
+            const u32x2 x = ld8(kq + 64 * kk), y = ld8(kq + 64 * kk + 32);
+            acc = T::mma16(u32x4{x[0], x[1], y[0], y[1]}, ld16(qq + 64 * kk), acc);
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i] *= kKeep ? pf[np][i] : p_factor(tile, i);
+          st8(lds_p + p_at + it * Scores::at(16) + group_at(4 * jt + lq),
+              u32x2{T::pack(acc[0], acc[1]), T::pack(acc[2], acc[3])});
         }
       }
       // O^T = S^T Q^T, then the rows' decay.  fp16: S meets Q scaled by a power of
       // two (its largest value to 2^14), so that neither a long memory's sums nor
       // small ones leave the type's range.
-      float up = 1.f, down = 1.f;
+      float up = inter_scale, down = 1.f;
       if constexpr (T::kId == 0) {
         float m = 0.f;
 #pragma unroll
         for (int dt = 0; dt < L::DT; ++dt)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(S[dt][i]));
-        m = wave_max(m);
+          for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(S[dt][i]));
+        m = __builtin_bit_cast(float, wave_max_nonneg(__builtin_bit_cast(int, m)));
         const int e = m > 0.f && m < __builtin_inff() ? min(max(exponent(m), -100), 100) : 14;
         down = pow2(14 - e);
-        up = pow2(e - 14) * pow2(-held);
+        up *= pow2(e - 14) * pow2(-held);
       }
-      o[0] = o[1] = f32x16{};
+#pragma unroll
+      for (int it = 0; it < 4; ++it) o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int dt = 0; dt < L::DT; dt += 2) {
+        u32x4 sf;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          sf[i] = T::pack(S[dt + i / 2][2 * (i & 1)] * down, S[dt + i / 2][2 * (i & 1) + 1] * down);
+#pragma unroll
+        for (int it = 0; it < 4; ++it)
+          o[it] = T::mma16(sf, ld16(lds_q + op_at + it * Tile::at(16) + 32 * dt), o[it]);
+      }
+#pragma unroll
+      for (int it = 0; it < 4; ++it) o[it] *= up * (kKeep ? rowf[it] : row_factor(it));
+    }
+
+    auto finish = [&]() {
+      __syncthreads();  // P is there
+      // O^T += V^T P^T
+#pragma unroll
+      for (int s = 0; s < kChunk / 32; ++s)
+#pragma unroll
+        for (int it = 2 * s; it < 4; ++it)
+          o[it] = T::mma16(vt[s], ld16(lds_p + p_at + it * Scores::at(16) + 64 * s + 16 * lq), o[it]);
+      if (a.out_f32) {
+        const rsrc_t rs = make_rsrc(static_cast<float*>(a.out) + batch * a.os[0] +
+                                        lowest(c, n) * a.os[1] + h * a.os[2],
+                                    (uint32_t)((n - 1) * a.os[1] + D) * 4u);
+#pragma unroll
+        for (int it = 0; it < 4; ++it)
+          __builtin_amdgcn_raw_buffer_store_b128(
+              __builtin_bit_cast(u32x4, o[it]), rs,
+              row_offset(16 * it + lc, n, step, 4 * (uint32_t)a.os[1], 4 * (16 * wave + 4 * lq)), 0,
+              0);
+      } else {
+        // Into V's columns of this wave, which no other wave reads.
+#pragma unroll
+        for (int it = 0; it < 4; ++it)
+          st8(lds_v + Tile::at(16 * it + lc) + 32 * wave + 8 * lq,
+              u32x2{T::pack(o[it][0], o[it][1]), T::pack(o[it][2], o[it][3])});
+      }
+    };
+    auto update = [&]() {
+      // S = l^n S + K^T (weight V).  The decay as S + S (l^n - 1): the factor's own
+      // rounding, which a slow decay would compound over hundreds of chunks, is then
+      // relative to the small difference.
 #pragma unroll
       for (int dt = 0; dt < L::DT; ++dt)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          u32x4 sf;
+        for (int i = 0; i < 4; ++i) S[dt][i] = fmaf(S[dt][i], dm1, S[dt][i]);
+      if constexpr (T::kId == 0) {
+        const int e = max_exponent(vt);
+        const int want = 13 - e - weight_top;
+        // Down where a term would overflow, up where eight bits would be lost.
+        if (e != kNone && (want < held || want > held + 8)) {
+          const float f = pow2(want - held);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sf[i] = T::pack(S[dt][8 * half + 2 * i] * down, S[dt][8 * half + 2 * i + 1] * down);
-#pragma unroll
-          for (int it = 0; it < 2; ++it)
-            o[it] = T::mma32(
-                sf, ld16(lds_q + op_at + it * Tile::at(32) + 64 * dt + 32 * half), o[it]);
-        }
-#pragma unroll
-      for (int it = 0; it < 2; ++it)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[it][i] *= rowf[it] * up;
-      __syncthreads();  // P is there
-    }
-
-    // S = l^n S + K^T (weight V), and O^T += V^T P^T on the way.  The decay as
-    // S + S (l^n - 1): the factor's own rounding, which a slow decay would
-    // compound over hundreds of chunks, is then relative to the small difference.
-#pragma unroll
-    for (int dt = 0; dt < L::DT; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) S[dt][i] = fmaf(S[dt][i], dm1, S[dt][i]);
-    u32x4 vts[kChunk / 16];
-#pragma unroll
-    for (int s = 0; s < kChunk / 16; ++s) vts[s] = read_transposed<Tile>(vt_p, s);
-    if constexpr (T::kId == 0) {
-      const int e = max_exponent(vts);
-      const int want = 13 - e - weight_top;
-      // Down where a term would overflow, up where eight bits would be lost.
-      if (e != kNone && (want < held || want > held + 8)) {
-        const float f = pow2(want - held);
-#pragma unroll
-        for (int dt = 0; dt < L::DT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) S[dt][i] *= f;
-        held = want;
-      }
-    }
-    const float hold = T::kId == 0 ? pow2(held) : 1.f;
-#pragma unroll
-    for (int s = 0; s < kChunk / 16; ++s) {
-      const u32x4 vt = vts[s];
-      if constexpr (!STATE_ONLY) {
-#pragma unroll
-        for (int it = s / 2; it < 2; ++it)
-          o[it] = T::mma32(vt, ld16(lds_p + p_at + it * Scores::at(32) + 32 * s + 16 * lh), o[it]);
-      }
-      float x[8];
-      const f32x4 w0 = *reinterpret_cast<const f32x4*>(weight + 16 * s + 8 * lh) * hold;
-      const f32x4 w1 = *reinterpret_cast<const f32x4*>(weight + 16 * s + 8 * lh + 4) * hold;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = T::lo(vt[i]) * (i < 2 ? w0[2 * i] : w1[2 * i - 4]);
-        x[2 * i + 1] = T::hi(vt[i]) * (i < 2 ? w0[2 * i + 1] : w1[2 * i - 3]);
-      }
-      u32x4 term[NT];
-      split_terms<T, NT>(x, term);
-#pragma unroll
-      for (int dt = 0; dt < L::DT; ++dt) {
-        const u32x4 kt = read_transposed<Tile>(kt_p + 64 * dt, s);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) S[dt] = T::mma32(kt, term[t], S[dt]);
-      }
-    }
-
-    if constexpr (!STATE_ONLY) {
-      const int64_t at = batch * a.os[0] + lowest(c, n) * a.os[1] + h * a.os[2];
-      const uint32_t size = a.out_f32 ? 4 : 2, row = size * (uint32_t)a.os[1];
-      const rsrc_t rs = make_rsrc(static_cast<char*>(a.out) + at * size,
-                                  (uint32_t)((n - 1) * a.os[1] + D) * size);
-#pragma unroll
-      for (int it = 0; it < 2; ++it) {
-        const int r = 32 * it + lr;
-        const uint32_t off = (uint32_t)(step > 0 ? r : n - 1 - r) * row + size * (32 * wave + 4 * lh);
-        if (a.out_f32) {
-#pragma unroll
-          for (int gi = 0; gi < 4; ++gi)
-            __builtin_amdgcn_raw_buffer_store_b128(
-                __builtin_bit_cast(u32x4, f32x4{o[it][4 * gi], o[it][4 * gi + 1], o[it][4 * gi + 2],
-                                                o[it][4 * gi + 3]}),
-                rs, r < n ? off + 32 * gi : 0xffffffffu, 0, 0);
-        } else {
-#pragma unroll
-          for (int gi = 0; gi < 4; ++gi)
-            __builtin_amdgcn_raw_buffer_store_b64(
-                u32x2{T::pack(o[it][4 * gi], o[it][4 * gi + 1]),
-                      T::pack(o[it][4 * gi + 2], o[it][4 * gi + 3])},
-                rs, r < n ? off + 16 * gi : 0xffffffffu, 0, 0);
+          for (int dt = 0; dt < L::DT; ++dt) S[dt] *= f;
+          held = want;
         }
       }
+      const float hold = T::kId == 0 ? pow2(held) : 1.f;
+#pragma unroll
+      for (int s = 0; s < kChunk / 32; ++s) {
+        float x[8];
+        const f32x4 w0 = *reinterpret_cast<const f32x4*>(weight + 32 * s + 4 * lq) * hold;
+        const f32x4 w1 = *reinterpret_cast<const f32x4*>(weight + 32 * s + 16 + 4 * lq) * hold;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[2 * i] = T::lo(vt[s][i]) * (i < 2 ? w0[2 * i] : w1[2 * i - 4]);
+          x[2 * i + 1] = T::hi(vt[s][i]) * (i < 2 ? w0[2 * i + 1] : w1[2 * i - 3]);
+        }
+        u32x4 term[NT];
+        split_terms<T, NT>(x, term);
+#pragma unroll
+        for (int dt = 0; dt < L::DT; ++dt) {
+          const u32x4 kt = read_transposed<Tile>(kt_p + 32 * dt, s);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) S[dt] = T::mma16(kt, term[t], S[dt]);
+        }
+      }
+    };
+    // The update stands before the barrier that P's readers need, where the waves
+    // that formed P's tiles are behind the others; at head_dim 256 there are no
+    // registers to keep O through it.
+    if constexpr (STATE_ONLY) {
+      update();
+    } else if constexpr (D < 256) {
+      update();
+      finish();
+    } else {
+      finish();
+      update();
     }
   }
 
@@ -559,23 +626,26 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, 2) void linear_kernel(LinPara
   if (STATE_ONLY) {
 #pragma unroll
     for (int dt = 0; dt < L::DT; ++dt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4*>(seg_state + state_image<D>(wave, dt, i, lane)) =
-            f32x4{S[dt][4 * i] * out, S[dt][4 * i + 1] * out, S[dt][4 * i + 2] * out,
-                  S[dt][4 * i + 3] * out};
-  } else if (!p.segmented && fin) {
+      *reinterpret_cast<f32x4*>(seg_state + state_image<D>(wave, dt, lane)) = S[dt] * out;
+    return;
+  }
+  if (!a.out_f32) {
+    __syncthreads();
+    const int c = (nrows - 1) / kChunk * kChunk;
+    write_rows(c, nrows - c, threadIdx.x);
+  }
+  float* fin = sg.seg == sg.nseg - 1 ? fin_of(p, a, sg.b, h) : nullptr;
+  if (fin) {
 #pragma unroll
     for (int dt = 0; dt < L::DT; ++dt)
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        fin[(32 * dt + 8 * (i / 4) + 4 * lh + i % 4) * D + col] = S[dt][i] * out;
+      for (int i = 0; i < 4; ++i) fin[(16 * dt + 4 * lq + i) * D + col] = S[dt][i] * out;
   }
 }
 
 // Joins the segments' states in order: each slot's own state becomes the state
-// before it, and the last sum the final state.  A thread holds four components, in
-// the workspace's layout (state_image): rows d .. d + 3 of column e.
+// before it.  A thread holds four components, in the workspace's layout
+// (state_image): rows d .. d + 3 of column e.
 template <int D>
 __global__ __launch_bounds__(256) void linear_scan_kernel(LinParams p) {
   constexpr int PARTS = D * D / 1024;
@@ -599,27 +669,20 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(LinParams p) {
   float* state = p.ws + ((blockIdx.y * total + first) * p.heads + h) * D * D + at;
   const int64_t next = (int64_t)p.heads * D * D;
   const float* init = init_of(p, a, b, h);
-  float* fin = fin_of(p, a, b, h);
-  const float g = decay_of(p, h);
-  const float dm1 = expm1f(g * (float)p.seglen);
+  const float decay = expm1f(decay_of(p, h) * (float)p.seglen);
   f32x4 S = {0.f, 0.f, 0.f, 0.f};
-  const int lane = at / 4 % 64, quad = at / 256 % 4, dt = at / 1024 % (D / 32);
-  const int d = 32 * dt + 8 * quad + 4 * (lane >> 5), e = 32 * (at / (32 * D)) + (lane & 31);
+  const int lane = at / 4 % 64, dt = at / 256 % (D / 16);
+  const int d = 16 * dt + 4 * (lane >> 4), e = 16 * (at / (16 * D)) + (lane & 15);
   if (init) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) S[i] = init[(d + i) * a.ird + e * a.icd];
   }
   for (int s = 0; s < nseg; ++s, state += next) {
     f32x4 u = {0.f, 0.f, 0.f, 0.f};
-    if (s < nseg - 1 || fin) u = *reinterpret_cast<const f32x4*>(state);
+    if (s < nseg - 1) u = *reinterpret_cast<const f32x4*>(state);
     *reinterpret_cast<f32x4*>(state) = S;
-    const float f = s < nseg - 1 ? dm1 : expm1f(g * (float)(len - s * p.seglen));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) S[i] = fmaf(S[i], f, S[i]) + u[i];
-  }
-  if (fin) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) fin[(d + i) * D + e] = S[i];
+    for (int i = 0; i < 4; ++i) S[i] = fmaf(S[i], decay, S[i]) + u[i];
   }
 }
 
@@ -711,43 +774,78 @@ __global__ __launch_bounds__(256) void linear_decode_kernel(fa_linear_decode_arg
 
 // ------------------------------------------------------------------ host
 
-// Rows of a segment: enough segments for every CU to hold two workgroups (four
-// of head_dim 64's half-size ones), none shorter than four chunks.
-int segment_rows(int64_t tokens, int64_t units, int D) {
-  const int64_t want = (int64_t)device_cu_count() * (D == 64 ? 4 : 2);
-  const int64_t n = units > 0 ? (want + units - 1) / units : 1;
-  int64_t rows = (tokens + n - 1) / n;
-  rows = (rows + kChunk - 1) / kChunk * kChunk;
-  return (int)std::max<int64_t>(rows, 4 * kChunk);
+// Microseconds of a launch whose `groups` workgroups walk `chunks` chunks each,
+// `per_cu` of them on a CU at a time: a chunk takes `lat` for one workgroup alone
+// and `mem` for each of those on a CU where memory is the bound.
+double launch_us(int64_t groups, int64_t chunks, int per_cu, double lat, double mem) {
+  const int64_t cus = device_cu_count(), full = groups / (cus * per_cu);
+  const int64_t rest = groups - full * cus * per_cu;
+  const double start = 4.0;
+  double t = full * (start + chunks * std::max(lat, per_cu * mem));
+  if (rest > 0) t += start + chunks * std::max(lat, (double)((rest + cus - 1) / cus) * mem);
+  return t;
+}
+
+// Rows of a segment.  More segments fill the GPU, and each costs a state formed
+// twice and carried through memory: the count with the least time by the model
+// above.  Its constants are MI355X measurements (us a chunk); it is within 15% of
+// the measured times of [4, 2048, 16, 128], [2, 8192, 16, 128] and one sequence of
+// 18688 rows at 1 to 32 segments, and picks the fastest or one within 5% of it.
+// tokens: of one sequence, or of all `seqs` packed ones, which end in a part of a
+// segment each.
+int segment_rows(int64_t tokens, int64_t units, int64_t seqs, int D) {
+  const int per_cu = D == 64 ? 3 : 1;
+  const double lat = D == 64 ? 2.1 : (D == 128 ? 3.5 : 8.0);
+  const double mem = D == 64 ? 1.8 : (D == 128 ? 3.6 : 7.2);
+  const double bytes_us = 4.0 * D * D / 5e6;  // a state once through memory
+  const int64_t chunks = (tokens + kChunk - 1) / kChunk;
+  double best = 0;
+  int64_t rows = chunks;
+  for (int64_t n = 1; n <= std::min<int64_t>(chunks, 64); ++n) {
+    const int64_t c = (chunks + n - 1) / n;
+    if (n > 1 && (chunks + c - 1) / c < n) continue;  // the same as fewer
+    const int64_t segments = std::max(n + (seqs - 1) / 2, seqs);
+    double t = launch_us(units * segments, c, per_cu, lat, mem);
+    if (n > 1)
+      t += launch_us(units * (segments - seqs), c, 2 * per_cu, 0.6 * lat, 0.5 * mem) +
+           units * n * (n <= max_added(D) ? 1 + n / 2 : 4) * bytes_us +
+           (n <= max_added(D) ? 0 : 5);
+    if (n == 1 || t < best) {
+      best = t;
+      rows = c;
+    }
+  }
+  return (int)(rows * kChunk);
 }
 
 // Cuts p's sequences; returns the slots in all.
 int64_t set_segments(LinParams& p, int D) {
-  // Packed: the sequences' lengths are on the device; as if all were one.
+  // (Packed: the sequences' lengths are on the device.)
   const int64_t units = (int64_t)p.heads * p.npass * (p.starts ? 1 : p.batch);
-  p.seglen = segment_rows(p.seqlen, units, D);
-  p.segmented = p.seglen < p.seqlen;
+  p.seglen = segment_rows(p.seqlen, units, p.starts ? p.batch : 1, D);
+  const int64_t most = ((int64_t)p.seqlen + p.seglen - 1) / p.seglen;
+  p.join = most == 1 ? kWhole : (most <= max_added(D) ? kAdded : kScanned);
   if (p.starts) {
     p.nseg = p.seqlen / p.seglen + p.batch;
     return p.nseg;
   }
-  p.nseg = (p.seqlen + p.seglen - 1) / p.seglen;
+  p.nseg = (int)most;
   return (int64_t)p.nseg * p.batch;
 }
 
 size_t state_bytes(const LinParams& p, int64_t slots, int D) {
-  return p.segmented ? (size_t)slots * p.npass * p.heads * D * D * sizeof(float) : 0;
+  return p.join != kWhole ? (size_t)slots * p.npass * p.heads * D * D * sizeof(float) : 0;
 }
 
 template <class T, int D>
 hipError_t launch_passes(LinParams& p, int64_t slots, hipStream_t st) {
   const dim3 grid((unsigned)(slots * p.heads), p.npass), block(LinShape<D>::THREADS);
-  if (p.segmented) {
+  if (p.join != kWhole)
     hipLaunchKernelGGL((linear_kernel<T, D, true>), grid, block, 0, st, p);
+  if (p.join == kScanned)
     hipLaunchKernelGGL((linear_scan_kernel<D>),
                        dim3((unsigned)(D * D / 1024 * p.batch * p.heads), p.npass), dim3(256), 0,
                        st, p);
-  }
   hipLaunchKernelGGL((linear_kernel<T, D, false>), grid, block, 0, st, p);
   return hipGetLastError();
 }
