@@ -39,6 +39,10 @@ struct Entries {
   decltype(&fa_linear_fwd_workspace_bytes) linear_workspace;
   decltype(&fa_linear_fwd) linear_fwd;
   decltype(&fa_linear_decode) linear_decode;
+  decltype(&fa_norm_rope_bwd_workspace_bytes) norm_rope_bwd_workspace;
+  decltype(&fa_norm_rope_bwd) norm_rope_bwd;
+  decltype(&fa_linear_bwd_workspace_bytes) linear_bwd_workspace;
+  decltype(&fa_linear_bwd) linear_bwd;
 } lib;
 
 struct Call {
@@ -429,6 +433,38 @@ const int64_t* long_index(PyObject* o, const Call& c, int64_t n) {
              : nullptr;
 }
 
+// {batch, seq, head} strides of a [B, S, H, D] or [T, H, D] tensor.
+void set_rows(int64_t (&dst)[3], const at::Tensor& t) {
+  const int64_t n = t.dim() - 1;
+  for (int64_t i = 0; i < n; ++i) dst[3 - n + i] = t.size(i) == 1 ? 0 : t.stride(i);
+}
+
+// Sizes and positions (None or a vector) of q / k, or of their gradients.
+template <class Args>
+bool rope_sizes(const at::Tensor& q, const at::Tensor& k, PyObject* positions, const Call& c,
+                Args* p) {
+  const int64_t d = q.dim();
+  for (int64_t i = 0; i < d; ++i)
+    if ((i != d - 2 && q.size(i) != k.size(i)) || !fits(q.size(i)) || !fits(k.size(i)))
+      return false;
+  if (positions != Py_None) {
+    p->positions = long_index(positions, c, q.size(d - 3));
+    if (!p->positions) return false;
+    p->pos_stride[1] = 1;
+  }
+  p->batch = d == 4 ? (int32_t)q.size(0) : 1;
+  p->seqlen = (int32_t)q.size(d - 3);
+  p->num_heads = (int32_t)q.size(d - 2);
+  p->num_heads_k = (int32_t)k.size(d - 2);
+  return true;
+}
+
+// A plain tensor [B, S, H, D] or [T, H, D].
+const at::Tensor* plain_heads(PyObject* o, const Call& c) {
+  const at::Tensor* t = plain(o, c, 4);
+  return t ? t : plain(o, c, 3);
+}
+
 // norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved, device, stream)
 //   -> (q_out, k_out) | status | None.  Positions: None or a vector.
 PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -436,25 +472,11 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Call c;
     fa_norm_rope_args p = {};
     if (n != 11 || !call_of(a[9], a[10], &c)) return none();
-    const at::Tensor *q = plain(a[0], c, 4), *k = plain(a[1], c, 4);
-    const bool dense = q != nullptr;
-    if (!dense) {
-      q = plain(a[0], c, 3);
-      k = plain(a[1], c, 3);
-    }
-    if (!q || !k || !half_code(*q, &p.dtype) || !rows_ready(*q) || !same_half(k, *q) ||
-        !rope_common(a[2], a[3], a[4], a[5], a[7], a[8], *q, c, &p))
+    const at::Tensor *q = plain_heads(a[0], c), *k = plain_heads(a[1], c);
+    if (!q || !k || q->dim() != k->dim() || !half_code(*q, &p.dtype) || !rows_ready(*q) ||
+        !same_half(k, *q) || !rope_common(a[2], a[3], a[4], a[5], a[7], a[8], *q, c, &p) ||
+        !rope_sizes(*q, *k, a[6], c, &p))
       return none();
-    const int64_t d = q->dim();
-    for (int64_t i = 0; i < d; ++i)
-      if (i != d - 2 && q->size(i) != k->size(i)) return none();
-    for (int64_t i = 0; i < d; ++i)
-      if (!fits(q->size(i)) || !fits(k->size(i))) return none();
-    if (a[6] != Py_None) {
-      p.positions = long_index(a[6], c, q->size(d - 3));
-      if (!p.positions) return none();
-      p.pos_stride[1] = 1;
-    }
     at::Tensor q_out, k_out;
     int status;
     {
@@ -465,22 +487,77 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.k = k->data_ptr();
       p.q_out = q_out.data_ptr();
       p.k_out = k_out.data_ptr();
-      auto put = [&](int64_t (&dst)[3], const at::Tensor& t) {
-        for (int64_t i = 0; i < d - 1; ++i)
-          dst[3 - (d - 1) + i] = t.size(i) == 1 ? 0 : t.stride(i);
-      };
-      put(p.q_stride, *q);
-      put(p.k_stride, *k);
-      put(p.qo_stride, q_out);
-      put(p.ko_stride, k_out);
-      p.batch = dense ? (int32_t)q->size(0) : 1;
-      p.seqlen = (int32_t)q->size(d - 3);
-      p.num_heads = (int32_t)q->size(d - 2);
-      p.num_heads_k = (int32_t)k->size(d - 2);
+      set_rows(p.q_stride, *q);
+      set_rows(p.k_stride, *k);
+      set_rows(p.qo_stride, q_out);
+      set_rows(p.ko_stride, k_out);
       status = lib.norm_rope(&p, c.stream);
     }
     if (status != FA_OK) return PyLong_FromLong(status);
     return Py_BuildValue("NN", THPVariable_Wrap(q_out), THPVariable_Wrap(k_out));
+  });
+}
+
+// norm_rope_bwd(q, k, dq_out, dk_out, cos, sin, q_weight, k_weight, positions, eps, interleaved,
+//               device, stream) -> (dq, dk, dq_weight, dk_weight) | status | None.
+// q / k and the weights' gradients are None where the weight is.
+PyObject* norm_rope_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Call c;
+    fa_norm_rope_bwd_args p = {};
+    if (n != 13 || !call_of(a[11], a[12], &c)) return none();
+    const at::Tensor *gq = plain_heads(a[2], c), *gk = plain_heads(a[3], c);
+    if (!gq || !gk || gq->dim() != gk->dim() || !half_code(*gq, &p.dtype) || !rows_ready(*gq) ||
+        !same_half(gk, *gq) || !rope_common(a[4], a[5], a[6], a[7], a[9], a[10], *gq, c, &p) ||
+        !rope_sizes(*gq, *gk, a[8], c, &p))
+      return none();
+    const at::Tensor *q = nullptr, *k = nullptr;
+    if (p.q_weight) {
+      q = plain_heads(a[0], c);
+      if (!same_half(q, *gq) || q->sizes() != gq->sizes()) return none();
+    }
+    if (p.k_weight) {
+      k = plain_heads(a[1], c);
+      if (!same_half(k, *gq) || k->sizes() != gk->sizes()) return none();
+    }
+    at::Tensor dq, dk, dqw, dkw;
+    int status;
+    {
+      NoGil no_gil;
+      dq = at::empty(gq->sizes(), gq->options().requires_grad(false));
+      dk = at::empty(gk->sizes(), dq.options());
+      const auto w = dq.options().dtype(p.weight_f32 ? at::kFloat : gq->scalar_type());
+      if (q) {
+        dqw = at::empty({p.head_dim}, w);
+        p.q = q->data_ptr();
+        set_rows(p.q_stride, *q);
+        p.dq_weight = dqw.data_ptr();
+      }
+      if (k) {
+        dkw = at::empty({p.head_dim}, w);
+        p.k = k->data_ptr();
+        set_rows(p.k_stride, *k);
+        p.dk_weight = dkw.data_ptr();
+      }
+      p.dq_out = gq->data_ptr();
+      p.dk_out = gk->data_ptr();
+      p.dq = dq.data_ptr();
+      p.dk = dk.data_ptr();
+      set_rows(p.dqo_stride, *gq);
+      set_rows(p.dko_stride, *gk);
+      set_rows(p.dq_stride, dq);
+      set_rows(p.dk_stride, dk);
+      const size_t bytes = lib.norm_rope_bwd_workspace(&p);
+      at::Tensor ws;
+      if (bytes) ws = at::empty({(int64_t)bytes}, dq.options().dtype(at::kByte));
+      status = lib.norm_rope_bwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, c.stream);
+    }
+    if (status != FA_OK) return PyLong_FromLong(status);
+    auto or_none = [](const at::Tensor& t) {
+      return t.defined() ? THPVariable_Wrap(t) : (Py_INCREF(Py_None), Py_None);
+    };
+    return Py_BuildValue("NNNN", THPVariable_Wrap(dq), THPVariable_Wrap(dk), or_none(dqw),
+                         or_none(dkw));
   });
 }
 
@@ -572,6 +649,137 @@ bool linear_common(PyObject* const* a, PyObject* slots_o, PyObject* scale, int64
   return true;
 }
 
+// Dense q [B, S, H, D], k, v [B, S, Hk, D] and log_decay [H].
+template <class Args>
+bool linear_dense(const at::Tensor* q, const at::Tensor* k, const at::Tensor* v, PyObject* decay,
+                  PyObject* scale, const Call& c, Args* p) {
+  const at::Tensor* g = plain(decay, c, 1);
+  if (!q || !half_code(*q, &p->dtype) || !rows_ready(*q) || !same_half(k, *q) ||
+      !same_half(v, *q) || k->sizes() != v->sizes() || k->size(0) != q->size(0) ||
+      k->size(1) != q->size(1) || k->size(3) != q->size(3) || !g || !number(scale, &p->scale))
+    return false;
+  const int64_t H = q->size(2), Hk = k->size(2), D = q->size(3), lim = int64_t(1) << 24;
+  if ((D != 64 && D != 128 && D != 256) || H % Hk != 0 || !fits(H) || !fits(q->size(0)) ||
+      !fits(q->size(1)) || q->stride(1) >= lim || k->stride(1) >= lim || v->stride(1) >= lim ||
+      g->scalar_type() != at::kFloat || g->size(0) != H || !g->is_contiguous() ||
+      g->requires_grad())
+    return false;
+  p->q = q->data_ptr();
+  p->k = k->data_ptr();
+  p->v = v->data_ptr();
+  p->log_decay = g->data_ptr<float>();
+  set_strides(p->q_stride, *q);
+  set_strides(p->k_stride, *k);
+  set_strides(p->v_stride, *v);
+  p->batch = (int32_t)q->size(0);
+  p->seqlen = (int32_t)q->size(1);
+  p->num_heads = (int32_t)H;
+  p->num_heads_k = (int32_t)Hk;
+  p->head_dim = (int32_t)D;
+  return true;
+}
+
+// None, or a contiguous fp32 [B, H, D, D] state of q's sizes: its data and strides.
+template <size_t N>
+bool state_of(PyObject* o, const at::Tensor& q, const Call& c, const float** data,
+              int64_t (&stride)[N]) {
+  if (o == Py_None) return true;
+  const at::Tensor* s = plain(o, c, 4);
+  if (!s || s->scalar_type() != at::kFloat || s->size(0) != q.size(0) ||
+      s->size(1) != q.size(2) || s->size(2) != q.size(3) || s->size(3) != q.size(3) ||
+      !s->is_contiguous() || reinterpret_cast<uintptr_t>(s->data_ptr()) % 16 != 0)
+    return false;
+  *data = s->data_ptr<float>();
+  set_strides(stride, *s);
+  return true;
+}
+
+// linear_dense_fwd(q, k, v, log_decay, scale, initial_state, want_final, device, stream)
+//   -> (out, final_state or None) | status | None
+PyObject* linear_dense_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Call c;
+    fa_linear_args p = {};
+    if (n != 9 || !call_of(a[7], a[8], &c)) return none();
+    const at::Tensor* q = plain(a[0], c, 4);
+    if (!linear_dense(q, plain(a[1], c, 4), plain(a[2], c, 4), a[3], a[4], c, &p) ||
+        !state_of(a[5], *q, c, &p.initial_state, p.is_stride))
+      return none();
+    const bool want_final = a[6] == Py_True;
+    at::Tensor out, fin;
+    int status;
+    {
+      NoGil no_gil;
+      out = at::empty(q->sizes(), q->options().requires_grad(false));
+      p.out = out.data_ptr();
+      set_strides(p.o_stride, out);
+      p.num_states = p.batch;
+      if (want_final) {
+        fin = at::empty({q->size(0), q->size(2), q->size(3), q->size(3)},
+                        out.options().dtype(at::kFloat));
+        p.final_state = fin.data_ptr<float>();
+        set_strides(p.fs_stride, fin);
+      }
+      const size_t bytes = lib.linear_workspace(&p);
+      at::Tensor ws;
+      if (bytes) ws = at::empty({(int64_t)bytes}, out.options().dtype(at::kByte));
+      status = lib.linear_fwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, c.stream);
+    }
+    if (status != FA_OK) return PyLong_FromLong(status);
+    PyObject* f = want_final ? THPVariable_Wrap(fin) : (Py_INCREF(Py_None), Py_None);
+    return Py_BuildValue("NN", THPVariable_Wrap(out), f);
+  });
+}
+
+// linear_dense_bwd(q, k, v, dout, log_decay, scale, initial_state, d_final_state,
+//                  want_d_initial, device, stream)
+//   -> (dq, dk, dv, d_initial_state or None) | status | None
+PyObject* linear_dense_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Call c;
+    fa_linear_bwd_args p = {};
+    if (n != 11 || !call_of(a[9], a[10], &c)) return none();
+    const at::Tensor *q = plain(a[0], c, 4), *k = plain(a[1], c, 4), *v = plain(a[2], c, 4),
+                     *g = plain(a[3], c, 4);
+    if (!linear_dense(q, k, v, a[4], a[5], c, &p) || !same_half(g, *q) ||
+        g->sizes() != q->sizes() || g->stride(1) >= (int64_t(1) << 24) ||
+        !state_of(a[6], *q, c, &p.initial_state, p.is_stride) ||
+        !state_of(a[7], *q, c, &p.d_final_state, p.fs_stride))
+      return none();
+    const bool want = a[8] == Py_True;
+    at::Tensor dq, dk, dv, ds;
+    int status;
+    {
+      NoGil no_gil;
+      dq = at::empty(q->sizes(), q->options().requires_grad(false));
+      dk = at::empty(k->sizes(), dq.options());
+      dv = at::empty(k->sizes(), dq.options());
+      p.dout = g->data_ptr();
+      p.dq = dq.data_ptr();
+      p.dk = dk.data_ptr();
+      p.dv = dv.data_ptr();
+      set_strides(p.do_stride, *g);
+      set_strides(p.dq_stride, dq);
+      set_strides(p.dk_stride, dk);
+      set_strides(p.dv_stride, dv);
+      if (want) {
+        ds = at::empty({q->size(0), q->size(2), q->size(3), q->size(3)},
+                       dq.options().dtype(at::kFloat));
+        p.d_initial_state = ds.data_ptr<float>();
+        set_strides(p.dis_stride, ds);
+      }
+      const size_t bytes = lib.linear_bwd_workspace(&p);
+      at::Tensor ws;
+      if (bytes) ws = at::empty({(int64_t)bytes}, dq.options().dtype(at::kByte));
+      status = lib.linear_bwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, c.stream);
+    }
+    if (status != FA_OK) return PyLong_FromLong(status);
+    PyObject* d = want ? THPVariable_Wrap(ds) : (Py_INCREF(Py_None), Py_None);
+    return Py_BuildValue("NNNN", THPVariable_Wrap(dq), THPVariable_Wrap(dk), THPVariable_Wrap(dv),
+                         d);
+  });
+}
+
 // linear_prefill(q, k, v, log_decay, state, query_start_loc, prefix_kv_lens, state_indices,
 //                scale, device, stream) -> out | status | None
 PyObject* linear_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -648,7 +856,7 @@ PyObject* linear_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // bind(...): the library's entry points, as addresses, in the order of Entries.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  constexpr int kEntries = 12;
+  constexpr int kEntries = 16;
   void* f[kEntries];
   if (n != kEntries) {
     PyErr_Format(PyExc_TypeError, "bind takes %d addresses", kEntries);
@@ -669,7 +877,11 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
          reinterpret_cast<decltype(lib.norm_rope_cache)>(f[8]),
          reinterpret_cast<decltype(lib.linear_workspace)>(f[9]),
          reinterpret_cast<decltype(lib.linear_fwd)>(f[10]),
-         reinterpret_cast<decltype(lib.linear_decode)>(f[11])};
+         reinterpret_cast<decltype(lib.linear_decode)>(f[11]),
+         reinterpret_cast<decltype(lib.norm_rope_bwd_workspace)>(f[12]),
+         reinterpret_cast<decltype(lib.norm_rope_bwd)>(f[13]),
+         reinterpret_cast<decltype(lib.linear_bwd_workspace)>(f[14]),
+         reinterpret_cast<decltype(lib.linear_bwd)>(f[15])};
   Py_RETURN_NONE;
 }
 
@@ -686,6 +898,9 @@ PyMethodDef methods[] = {method<bind>("bind"),
                          method<cache_write>("cache_write"),
                          method<norm_rope>("norm_rope"),
                          method<norm_rope_cache>("norm_rope_cache"),
+                         method<norm_rope_bwd>("norm_rope_bwd"),
+                         method<linear_dense_fwd>("linear_dense_fwd"),
+                         method<linear_dense_bwd>("linear_dense_bwd"),
                          method<linear_prefill>("linear_prefill"),
                          method<linear_decode>("linear_decode"),
                          {nullptr, nullptr, 0, nullptr}};

@@ -125,6 +125,9 @@ def _launch_fwd(a, device):
 # ------------------------------------------------------------------ training
 
 def _forward(q, k, v, log_decay, scale, initial_state, want_final):
+    done = _native.linear_dense_fwd(q, k, v, log_decay, scale, initial_state, want_final)
+    if done is not None:
+        return done
     H, Hk, D = _check_qkv(q, k, v, ("batch", "seqlen", "heads", "head_dim"))
     B, S = q.shape[:2]
     _check_decay(log_decay, H)
@@ -158,6 +161,10 @@ def _forward(q, k, v, log_decay, scale, initial_state, want_final):
 
 def _backward(q, k, v, dout, log_decay, scale, initial_state, d_final, want_d_initial):
     """(dq, dk, dv, d_initial_state or None)."""
+    done = _native.linear_dense_bwd(q, k, v, dout, log_decay, scale, initial_state, d_final,
+                                    want_d_initial)
+    if done is not None:
+        return done
     B, S, H, D = q.shape
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     if B == 0 or S == 0:

@@ -21,7 +21,8 @@ _ENTRIES = ("fa_fwd", "fa_decode_workspace_bytes", "fa_paged_decode",
             "fa_paged_prefill_num_splits", "fa_paged_prefill_splitkv_workspace_bytes",
             "fa_paged_prefill_splitkv", "fa_reshape_and_cache", "fa_norm_rope",
             "fa_norm_rope_and_cache", "fa_linear_fwd_workspace_bytes", "fa_linear_fwd",
-            "fa_linear_decode")
+            "fa_linear_decode", "fa_norm_rope_bwd_workspace_bytes", "fa_norm_rope_bwd",
+            "fa_linear_bwd_workspace_bytes", "fa_linear_bwd")
 _lock = threading.Lock()
 _module = None
 _missing = False  # load() failed: the Python path takes every call
@@ -113,6 +114,21 @@ def norm_rope(q, *args):
 def norm_rope_cache(q, *args):
     """q_out, or None."""
     return _run("norm_rope_cache", "fa_norm_rope_and_cache", q, (q, *args))
+
+
+def norm_rope_bwd(q, k, dq_out, *args):
+    """(dq, dk, dq_weight or None, dk_weight or None), or None."""
+    return _run("norm_rope_bwd", "fa_norm_rope_bwd", dq_out, (q, k, dq_out, *args))
+
+
+def linear_dense_fwd(q, *args):
+    """(out, final_state or None), or None."""
+    return _run("linear_dense_fwd", "fa_linear_fwd", q, (q, *args))
+
+
+def linear_dense_bwd(q, *args):
+    """(dq, dk, dv, d_initial_state or None), or None."""
+    return _run("linear_dense_bwd", "fa_linear_bwd", q, (q, *args))
 
 
 def linear_prefill(q, *args):

@@ -144,6 +144,10 @@ def _forward(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved):
 
 def _backward(q, k, dq_out, dk_out, cos, sin, q_weight, k_weight, positions, eps, interleaved):
     """q / k (None where the weight is None) and the outputs' gradients -> the gradients."""
+    done = _native.norm_rope_bwd(q, k, dq_out, dk_out, cos, sin, q_weight, k_weight, positions,
+                                 eps, interleaved)
+    if done is not None:
+        return done
     dq_out, dk_out = rows_ready(dq_out), rows_ready(dk_out)
     dq = torch.empty(dq_out.shape, dtype=dq_out.dtype, device=dq_out.device)
     dk = torch.empty(dk_out.shape, dtype=dk_out.dtype, device=dk_out.device)
