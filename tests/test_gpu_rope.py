@@ -297,7 +297,7 @@ def test_native_and_python_paths_agree(monkeypatch):
     q, k = randn(g, 2, 30, 4, 128).to(DEV), randn(g, 2, 30, 2, 128).to(DEV)
     cos, sin = (t.to(DEV) for t in table(30, 64))
     w = torch.ones(128, device=DEV)
-    assert _native.norm_rope(q, k, cos, sin, w, None, None, 1e-6, False) is not None
+    assert _native.norm_rope(q, k, cos, sin, w, None, None, 1e-6, False, False) is not None
     kc, vc = (torch.zeros(5, 16, 2, 128, dtype=q.dtype, device=DEV) for _ in range(2))
     slots = torch.arange(60, device=DEV)
     flat = [t.reshape(60, -1, 128) for t in (q, k)]

@@ -205,7 +205,7 @@ def test_linear_refusals():
 
 def test_native_hands_back_what_is_not_plain():
     m, t = _native.load(), h(2, 4, 64)
-    assert m.norm_rope(t, t, t, t, None, None, None, 1e-6, False, 0, 0) is None
+    assert m.norm_rope(t, t, t, t, None, None, None, 1e-6, False, False, 0, 0) is None
     assert m.norm_rope_cache(t, t, t, t, t, t, t, t, t, None, None, 1e-6, False, 0, 0) is None
     assert m.linear_prefill(t, t, t, t, t, t, t, None, None, 0, 0) is None
     assert m.linear_decode(t, t, t, t, t, None, None, 0, 0) is None

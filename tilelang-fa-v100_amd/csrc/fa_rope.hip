@@ -121,7 +121,7 @@ __device__ __forceinline__ Lane lane_chunks(const Params& p, int c) {
   return l;
 }
 
-__device__ __forceinline__ void load8(const void* w, int f32, int chunk, bool there, int dtype_bf16,
+__device__ __forceinline__ void load8(const void* w, int f32, int chunk, bool there, int bf16,
                                       float (&out)[8]) {
   if (!there) {
 #pragma unroll
@@ -130,12 +130,16 @@ __device__ __forceinline__ void load8(const void* w, int f32, int chunk, bool th
   }
   if (f32) {
     const float* p = static_cast<const float*>(w) + 8 * chunk;
+    const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = p[i];
+    for (int i = 0; i < 4; ++i) {
+      out[i] = x[i];
+      out[4 + i] = y[i];
+    }
     return;
   }
   const u32x4 v = ld16(static_cast<const uint16_t*>(w) + 8 * chunk);
-  if (dtype_bf16)
+  if (bf16)
     unpack<BFloat16>(v, out);
   else
     unpack<Half>(v, out);
@@ -209,78 +213,64 @@ __device__ __forceinline__ int64_t offset_of(const int64_t (&s)[3], const Token&
   return k.b * s[0] + k.s * s[1] + k.h * s[2];
 }
 
-// U rows a group: their loads go out together.
-template <class T, int LPR, int U, bool CACHE>
+// One row a group of lanes.  (Two to four rows a group, their loads issued together:
+// within 3%, [2, 8192, 32 + 8, 128] 68-72 us; the waves of a CU overlap enough.)
+template <class T, int LPR, bool CACHE>
 __global__ __launch_bounds__(kThreads) void norm_rope_kernel(Params p) {
-  constexpr int G = kThreads / LPR;  // rows of a workgroup at a time
+  constexpr int G = kThreads / LPR;  // rows of a workgroup
   uint32_t blk = blockIdx.x;
   const bool is_q = blk < p.q.blocks;
   const bool is_v = CACHE && blk >= p.q.blocks + p.k.blocks;
   const Rows& R = is_q ? p.q : (is_v ? p.v : p.k);
   blk -= is_q ? 0 : (is_v ? p.q.blocks + p.k.blocks : p.q.blocks);
+  const uint32_t row = blk * G + threadIdx.x / LPR;
+  if (row >= R.count) return;
   const int c = threadIdx.x % LPR;
   const Lane l = lane_chunks(p, c);
-  const bool norm = R.w != nullptr;
-  float wa[8], wb[8];
-  if (norm) {
-    load8(R.w, p.weight_f32, l.ca, l.has_a, T::kId, wa);
-    load8(R.w, p.weight_f32, l.cb, l.has_b, T::kId, wb);
+  const Token k = token_of(p, R, row);
+  const uint16_t* xp = R.x + offset_of(R.xs, k);
+  u32x4 xa = {0, 0, 0, 0}, xb = xa;
+  if (l.has_a) xa = ld16(xp + 8 * l.ca);
+  if (l.has_b) xb = ld16(xp + 8 * l.cb);
+  uint16_t* out;
+  if (CACHE && !is_q) {
+    const int64_t slot = p.slots[k.t];
+    if (slot < 0 || slot >= p.max_slot) return;
+    const int64_t page = p.max_slot <= 0x7fffffff ? (int64_t)p.page.quot((uint32_t)slot)
+                                                  : slot / p.page_size;
+    out = R.y + page * R.ys[0] + (slot - page * p.page_size) * R.ys[1] + k.h * R.ys[2];
+  } else {
+    out = R.y + offset_of(R.ys, k);
   }
-  const uint32_t row0 = blk * (G * U) + threadIdx.x / LPR;
-  u32x4 xa[U], xb[U];
-  uint16_t* out[U];
-  int64_t pos[U];
+  if (!is_v) {
+    const int64_t pos = position_of(p, k);
+    float a[8], b[8], cs[8], sn[8];
+    if (l.turns && pos >= 0) load_turn(p, pos, c, cs, sn);
+    unpack<T>(xa, a);
+    unpack<T>(xb, b);
+    if (R.w) {
+      float wa[8], wb[8];
+      load8(R.w, p.weight_f32, l.ca, l.has_a, T::kId, wa);
+      load8(R.w, p.weight_f32, l.cb, l.has_b, T::kId, wb);
+      const float sum = row_sum<LPR>(dot8(b, b, dot8(a, a, 0.f)));
+      const float r = rsqrtf(fmaf(sum, p.inv_d, p.eps));
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t row = row0 + u * G;
-    out[u] = nullptr;
-    xa[u] = xb[u] = u32x4{0, 0, 0, 0};
-    pos[u] = -1;
-    if (row >= R.count) continue;
-    const Token k = token_of(p, R, row);
-    const uint16_t* xp = R.x + offset_of(R.xs, k);
-    if (l.has_a) xa[u] = ld16(xp + 8 * l.ca);
-    if (l.has_b) xb[u] = ld16(xp + 8 * l.cb);
-    if (!is_v) pos[u] = position_of(p, k);
-    if (CACHE && !is_q) {
-      const int64_t slot = p.slots[k.t];
-      if (slot < 0 || slot >= p.max_slot) continue;
-      const int64_t page = p.max_slot <= 0x7fffffff ? (int64_t)p.page.quot((uint32_t)slot)
-                                                    : slot / p.page_size;
-      out[u] = R.y + page * R.ys[0] + (slot - page * p.page_size) * R.ys[1] + k.h * R.ys[2];
-    } else {
-      out[u] = R.y + offset_of(R.ys, k);
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (!out[u]) continue;
-    if (!is_v) {
-      float a[8], b[8], cs[8], sn[8];
-      if (l.turns && pos[u] >= 0) load_turn(p, pos[u], c, cs, sn);
-      unpack<T>(xa[u], a);
-      unpack<T>(xb[u], b);
-      if (norm) {
-        const float sum = row_sum<LPR>(dot8(b, b, dot8(a, a, 0.f)));
-        const float r = rsqrtf(fmaf(sum, p.inv_d, p.eps));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          a[i] *= r * wa[i];
-          b[i] *= r * wb[i];
-        }
+      for (int i = 0; i < 8; ++i) {
+        a[i] *= r * wa[i];
+        b[i] *= r * wb[i];
       }
-      if (pos[u] < 0) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
-      } else if (l.turns) {
-        turn<false>(p.interleaved, cs, sn, a, b);
-      }
-      xa[u] = pack8<T>(a);
-      xb[u] = pack8<T>(b);
     }
-    if (l.has_a) st16(out[u] + 8 * l.ca, xa[u]);
-    if (l.has_b) st16(out[u] + 8 * l.cb, xb[u]);
+    if (pos < 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+    } else if (l.turns) {
+      turn<false>(p.interleaved, cs, sn, a, b);
+    }
+    xa = pack8<T>(a);
+    xb = pack8<T>(b);
   }
+  if (l.has_a) st16(out + 8 * l.ca, xa);
+  if (l.has_b) st16(out + 8 * l.cb, xb);
 }
 
 // dx of every row; with a weight, the workgroup's sum of g x r over its rows goes
@@ -431,23 +421,12 @@ void set_common(Params& p, const Args& a, int seqlen) {
 template <class T, int LPR, bool CACHE>
 hipError_t launch_rows(Params& p, hipStream_t st) {
   constexpr int G = kThreads / LPR;
-  const uint64_t rows = (uint64_t)p.q.count + p.k.count + p.v.count;
-  auto grid = [&](int U) {
-    uint32_t n = 0;
-    for (Rows* r : {&p.q, &p.k, &p.v}) {
-      r->blocks = (uint32_t)(((uint64_t)r->count + G * U - 1) / (G * U));
-      n += r->blocks;
-    }
-    return n;
-  };
-  // Four rows a group where that still gives every CU four workgroups.
-  if (rows >= (uint64_t)G * 4 * 4 * device_cu_count()) {
-    const uint32_t n = grid(4);
-    hipLaunchKernelGGL((norm_rope_kernel<T, LPR, 4, CACHE>), dim3(n), dim3(kThreads), 0, st, p);
-  } else {
-    const uint32_t n = grid(1);
-    hipLaunchKernelGGL((norm_rope_kernel<T, LPR, 1, CACHE>), dim3(n), dim3(kThreads), 0, st, p);
+  uint32_t n = 0;
+  for (Rows* r : {&p.q, &p.k, &p.v}) {
+    r->blocks = (uint32_t)(((uint64_t)r->count + G - 1) / G);
+    n += r->blocks;
   }
+  hipLaunchKernelGGL((norm_rope_kernel<T, LPR, CACHE>), dim3(n), dim3(kThreads), 0, st, p);
   return hipGetLastError();
 }
 

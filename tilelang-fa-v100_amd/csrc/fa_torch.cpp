@@ -13,14 +13,27 @@
 // Python path, which converts, copies or raises, takes the call.  Otherwise
 // the result is the outputs, or the library's negative status for the caller
 // to raise.  Nothing is kept between calls except the library's entry points.
+//
+// The norm-and-rotation and linear-attention training calls put their own nodes
+// into the autograd graph: a Python Function's backward runs in the engine's thread
+// and waits there for the interpreter lock, ~50 us of a ~110 us step whose GPU work
+// took 77 us.
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 
 #include <climits>
 #include <cmath>
+#include <memory>
+#include <mutex>
 
 #include "fa355.h"
 
@@ -465,33 +478,182 @@ const at::Tensor* plain_heads(PyObject* o, const Call& c) {
   return t ? t : plain(o, c, 3);
 }
 
-// norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved, device, stream)
-//   -> (q_out, k_out) | status | None.  Positions: None or a vector.
+// fa_norm_rope on checked tensors (p holds what rope_common and rope_sizes set).
+int rope_forward(fa_norm_rope_args p, const at::Tensor& q, const at::Tensor& k, void* stream,
+                 at::Tensor* q_out, at::Tensor* k_out) {
+  *q_out = at::empty(q.sizes(), q.options().requires_grad(false));
+  *k_out = at::empty(k.sizes(), q_out->options());
+  p.q = q.data_ptr();
+  p.k = k.data_ptr();
+  p.q_out = q_out->data_ptr();
+  p.k_out = k_out->data_ptr();
+  set_rows(p.q_stride, q);
+  set_rows(p.k_stride, k);
+  set_rows(p.qo_stride, *q_out);
+  set_rows(p.ko_stride, *k_out);
+  return lib.norm_rope(&p, stream);
+}
+
+struct RopeGrads {
+  at::Tensor dq, dk, dqw, dkw;
+};
+// fa_norm_rope_bwd: gq, gk the outputs' gradients, q and k (read where their weight is).
+int rope_backward(fa_norm_rope_bwd_args p, const at::Tensor& q, const at::Tensor& k,
+                  const at::Tensor& gq, const at::Tensor& gk, void* stream, RopeGrads* r) {
+  r->dq = at::empty(gq.sizes(), gq.options().requires_grad(false));
+  r->dk = at::empty(gk.sizes(), r->dq.options());
+  const auto w = r->dq.options().dtype(p.weight_f32 ? at::kFloat : gq.scalar_type());
+  if (p.q_weight) {
+    r->dqw = at::empty({p.head_dim}, w);
+    p.q = q.data_ptr();
+    set_rows(p.q_stride, q);
+    p.dq_weight = r->dqw.data_ptr();
+  }
+  if (p.k_weight) {
+    r->dkw = at::empty({p.head_dim}, w);
+    p.k = k.data_ptr();
+    set_rows(p.k_stride, k);
+    p.dk_weight = r->dkw.data_ptr();
+  }
+  p.dq_out = gq.data_ptr();
+  p.dk_out = gk.data_ptr();
+  p.dq = r->dq.data_ptr();
+  p.dk = r->dk.data_ptr();
+  set_rows(p.dqo_stride, gq);
+  set_rows(p.dko_stride, gk);
+  set_rows(p.dq_stride, r->dq);
+  set_rows(p.dk_stride, r->dk);
+  const size_t bytes = lib.norm_rope_bwd_workspace(&p);
+  at::Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, r->dq.options().dtype(at::kByte));
+  return lib.norm_rope_bwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, stream);
+}
+
+// What a node of this file shares: the stream its forward ran on, which is the one
+// the engine makes current for its backward.
+struct FaNode : torch::autograd::Node {
+  void* stream = nullptr;
+  std::mutex lock;
+
+  // An output's gradient as the kernels take it: zeros where there is none.
+  static at::Tensor ready(const at::Tensor& g, at::IntArrayRef size, const at::TensorOptions& o) {
+    if (!g.defined()) return at::zeros(size, o);
+    at::Tensor t = g.scalar_type() == o.dtype().toScalarType() ? g : g.to(o.dtype());
+    return rows_ready(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+  }
+  // The gradients, which themselves have none: differentiating them is an error.
+  static torch::autograd::variable_list once(torch::autograd::variable_list&& out,
+                                             const torch::autograd::variable_list& grads) {
+    bool again = false;
+    for (const auto& g : grads) again |= g.defined() && g.requires_grad();
+    if (!again || !at::GradMode::is_enabled()) return std::move(out);
+    auto stop = std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a function that can be differentiated once",
+        (int64_t)out.size());
+    for (auto& t : out)
+      if (t.defined()) t = t.detach().set_requires_grad(true);
+    return (*stop)(std::move(out));
+  }
+};
+
+struct RopeNode : FaNode {
+  torch::autograd::SavedVariable q, k, cos, sin, qw, kw, pos;
+  bool has_q = false, has_k = false, has_pos = false;
+  std::vector<int64_t> q_size, k_size;
+  at::TensorOptions options;
+  fa_norm_rope_args p = {};
+
+  std::string name() const override { return "QkNormRopeBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> hold(lock);
+    for (auto* v : {&q, &k, &cos, &sin, &qw, &kw, &pos}) v->reset_data();
+  }
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> hold(lock);
+    at::Tensor c = cos.unpack(), s = sin.unpack(), x, y, a, b, t;
+    if (has_q) x = q.unpack(), a = qw.unpack();
+    if (has_k) y = k.unpack(), b = kw.unpack();
+    if (has_pos) t = pos.unpack();
+    RopeGrads r;
+    {
+      at::NoGradGuard none;
+      const at::Tensor gq = ready(grads[0], q_size, options), gk = ready(grads[1], k_size, options);
+      fa_norm_rope_bwd_args n = {};
+      n.q_weight = has_q ? a.data_ptr() : nullptr;
+      n.k_weight = has_k ? b.data_ptr() : nullptr;
+      n.cos = c.data_ptr<float>();
+      n.sin = s.data_ptr<float>();
+      n.positions = has_pos ? t.data_ptr<int64_t>() : nullptr;
+      for (int i = 0; i < 2; ++i) {
+        n.table_stride[i] = p.table_stride[i];
+        n.pos_stride[i] = p.pos_stride[i];
+      }
+      n.num_positions = p.num_positions;
+      n.batch = p.batch;
+      n.seqlen = p.seqlen;
+      n.num_heads = p.num_heads;
+      n.num_heads_k = p.num_heads_k;
+      n.head_dim = p.head_dim;
+      n.rotary_dim = p.rotary_dim;
+      n.interleaved = p.interleaved;
+      n.weight_f32 = p.weight_f32;
+      n.dtype = p.dtype;
+      n.eps = p.eps;
+      const int status = rope_backward(n, x, y, gq, gk, stream, &r);
+      TORCH_CHECK(status == FA_OK, "fa_norm_rope_bwd: status ", status);
+    }
+    return once({r.dq, r.dk, r.dqw, r.dkw}, grads);
+  }
+};
+
+at::Tensor or_undefined(PyObject* o) {
+  return o == Py_None ? at::Tensor() : THPVariable_Unpack(o);
+}
+
+// norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved, with_grad,
+//           device, stream) -> (q_out, k_out) | status | None.  Positions: None or a vector.
+// with_grad: the outputs have a node in the autograd graph.
 PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Call c;
     fa_norm_rope_args p = {};
-    if (n != 11 || !call_of(a[9], a[10], &c)) return none();
+    if (n != 12 || !call_of(a[10], a[11], &c)) return none();
     const at::Tensor *q = plain_heads(a[0], c), *k = plain_heads(a[1], c);
     if (!q || !k || q->dim() != k->dim() || !half_code(*q, &p.dtype) || !rows_ready(*q) ||
         !same_half(k, *q) || !rope_common(a[2], a[3], a[4], a[5], a[7], a[8], *q, c, &p) ||
         !rope_sizes(*q, *k, a[6], c, &p))
       return none();
+    const bool with_grad = a[9] == Py_True;
+    const at::Tensor cos = or_undefined(a[2]), sin = or_undefined(a[3]), qw = or_undefined(a[4]),
+                     kw = or_undefined(a[5]), pos = or_undefined(a[6]);
     at::Tensor q_out, k_out;
     int status;
     {
       NoGil no_gil;
-      q_out = at::empty(q->sizes(), q->options().requires_grad(false));
-      k_out = at::empty(k->sizes(), q_out.options());
-      p.q = q->data_ptr();
-      p.k = k->data_ptr();
-      p.q_out = q_out.data_ptr();
-      p.k_out = k_out.data_ptr();
-      set_rows(p.q_stride, *q);
-      set_rows(p.k_stride, *k);
-      set_rows(p.qo_stride, q_out);
-      set_rows(p.ko_stride, k_out);
-      status = lib.norm_rope(&p, c.stream);
+      status = rope_forward(p, *q, *k, c.stream, &q_out, &k_out);
+      if (status == FA_OK && with_grad) {
+        auto node = std::shared_ptr<RopeNode>(new RopeNode(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(*q, *k, qw, kw));
+        node->stream = c.stream;
+        node->p = p;
+        node->q_size = q->sizes().vec();
+        node->k_size = k->sizes().vec();
+        node->options = q_out.options();
+        using torch::autograd::SavedVariable;
+        if ((node->has_q = qw.defined())) {
+          node->q = SavedVariable(*q, false);
+          node->qw = SavedVariable(qw, false);
+        }
+        if ((node->has_k = kw.defined())) {
+          node->k = SavedVariable(*k, false);
+          node->kw = SavedVariable(kw, false);
+        }
+        if ((node->has_pos = pos.defined())) node->pos = SavedVariable(pos, false);
+        node->cos = SavedVariable(cos, false);
+        node->sin = SavedVariable(sin, false);
+        torch::autograd::set_history(q_out, node);
+        torch::autograd::set_history(k_out, node);
+      }
     }
     if (status != FA_OK) return PyLong_FromLong(status);
     return Py_BuildValue("NN", THPVariable_Wrap(q_out), THPVariable_Wrap(k_out));
@@ -511,53 +673,29 @@ PyObject* norm_rope_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !same_half(gk, *gq) || !rope_common(a[4], a[5], a[6], a[7], a[9], a[10], *gq, c, &p) ||
         !rope_sizes(*gq, *gk, a[8], c, &p))
       return none();
-    const at::Tensor *q = nullptr, *k = nullptr;
+    at::Tensor q, k;
     if (p.q_weight) {
-      q = plain_heads(a[0], c);
-      if (!same_half(q, *gq) || q->sizes() != gq->sizes()) return none();
+      const at::Tensor* t = plain_heads(a[0], c);
+      if (!same_half(t, *gq) || t->sizes() != gq->sizes()) return none();
+      q = *t;
     }
     if (p.k_weight) {
-      k = plain_heads(a[1], c);
-      if (!same_half(k, *gq) || k->sizes() != gk->sizes()) return none();
+      const at::Tensor* t = plain_heads(a[1], c);
+      if (!same_half(t, *gq) || t->sizes() != gk->sizes()) return none();
+      k = *t;
     }
-    at::Tensor dq, dk, dqw, dkw;
+    RopeGrads r;
     int status;
     {
       NoGil no_gil;
-      dq = at::empty(gq->sizes(), gq->options().requires_grad(false));
-      dk = at::empty(gk->sizes(), dq.options());
-      const auto w = dq.options().dtype(p.weight_f32 ? at::kFloat : gq->scalar_type());
-      if (q) {
-        dqw = at::empty({p.head_dim}, w);
-        p.q = q->data_ptr();
-        set_rows(p.q_stride, *q);
-        p.dq_weight = dqw.data_ptr();
-      }
-      if (k) {
-        dkw = at::empty({p.head_dim}, w);
-        p.k = k->data_ptr();
-        set_rows(p.k_stride, *k);
-        p.dk_weight = dkw.data_ptr();
-      }
-      p.dq_out = gq->data_ptr();
-      p.dk_out = gk->data_ptr();
-      p.dq = dq.data_ptr();
-      p.dk = dk.data_ptr();
-      set_rows(p.dqo_stride, *gq);
-      set_rows(p.dko_stride, *gk);
-      set_rows(p.dq_stride, dq);
-      set_rows(p.dk_stride, dk);
-      const size_t bytes = lib.norm_rope_bwd_workspace(&p);
-      at::Tensor ws;
-      if (bytes) ws = at::empty({(int64_t)bytes}, dq.options().dtype(at::kByte));
-      status = lib.norm_rope_bwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, c.stream);
+      status = rope_backward(p, q, k, *gq, *gk, c.stream, &r);
     }
     if (status != FA_OK) return PyLong_FromLong(status);
     auto or_none = [](const at::Tensor& t) {
       return t.defined() ? THPVariable_Wrap(t) : (Py_INCREF(Py_None), Py_None);
     };
-    return Py_BuildValue("NNNN", THPVariable_Wrap(dq), THPVariable_Wrap(dk), or_none(dqw),
-                         or_none(dkw));
+    return Py_BuildValue("NNNN", THPVariable_Wrap(r.dq), THPVariable_Wrap(r.dk), or_none(r.dqw),
+                         or_none(r.dkw));
   });
 }
 
@@ -694,18 +832,107 @@ bool state_of(PyObject* o, const at::Tensor& q, const Call& c, const float** dat
   return true;
 }
 
-// linear_dense_fwd(q, k, v, log_decay, scale, initial_state, want_final, device, stream)
-//   -> (out, final_state or None) | status | None
+struct LinearGrads {
+  at::Tensor dq, dk, dv, ds;
+};
+// fa_linear_bwd on checked tensors (p holds what linear_dense and state_of set).
+int linear_backward(fa_linear_bwd_args p, const at::Tensor& q, const at::Tensor& k,
+                    const at::Tensor& g, bool want_state, void* stream, LinearGrads* r) {
+  r->dq = at::empty(q.sizes(), q.options().requires_grad(false));
+  r->dk = at::empty(k.sizes(), r->dq.options());
+  r->dv = at::empty(k.sizes(), r->dq.options());
+  p.dout = g.data_ptr();
+  p.dq = r->dq.data_ptr();
+  p.dk = r->dk.data_ptr();
+  p.dv = r->dv.data_ptr();
+  set_strides(p.do_stride, g);
+  set_strides(p.dq_stride, r->dq);
+  set_strides(p.dk_stride, r->dk);
+  set_strides(p.dv_stride, r->dv);
+  if (want_state) {
+    r->ds = at::empty({q.size(0), q.size(2), q.size(3), q.size(3)},
+                      r->dq.options().dtype(at::kFloat));
+    p.d_initial_state = r->ds.data_ptr<float>();
+    set_strides(p.dis_stride, r->ds);
+  }
+  const size_t bytes = lib.linear_bwd_workspace(&p);
+  at::Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, r->dq.options().dtype(at::kByte));
+  return lib.linear_bwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, stream);
+}
+
+struct LinearNode : FaNode {
+  torch::autograd::SavedVariable q, k, v, decay, init;
+  bool has_init = false, want_init = false;
+  std::vector<int64_t> state_size;
+  fa_linear_args p = {};
+
+  std::string name() const override { return "LinearAttnBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> hold(lock);
+    for (auto* x : {&q, &k, &v, &decay, &init}) x->reset_data();
+  }
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
+    std::lock_guard<std::mutex> hold(lock);
+    const at::Tensor tq = q.unpack(), tk = k.unpack(), tv = v.unpack(), td = decay.unpack();
+    at::Tensor ti;
+    if (has_init) ti = init.unpack();
+    LinearGrads r;
+    {
+      at::NoGradGuard none;
+      at::Tensor g = ready(grads[0], tq.sizes(), tq.options().requires_grad(false));
+      if (g.stride(1) >= (int64_t(1) << 24)) g = g.clone(at::MemoryFormat::Contiguous);
+      at::Tensor ds;
+      if (grads.size() > 1 && grads[1].defined()) {
+        ds = grads[1].to(at::kFloat).contiguous();
+        if (reinterpret_cast<uintptr_t>(ds.data_ptr()) % 16 != 0)
+          ds = ds.clone(at::MemoryFormat::Contiguous);
+      }
+      fa_linear_bwd_args n = {};
+      n.q = tq.data_ptr();
+      n.k = tk.data_ptr();
+      n.v = tv.data_ptr();
+      n.log_decay = td.data_ptr<float>();
+      for (int i = 0; i < 3; ++i) {
+        n.q_stride[i] = p.q_stride[i];
+        n.k_stride[i] = p.k_stride[i];
+        n.v_stride[i] = p.v_stride[i];
+      }
+      if (has_init) {
+        n.initial_state = ti.data_ptr<float>();
+        set_strides(n.is_stride, ti);
+      }
+      if (ds.defined()) {
+        n.d_final_state = ds.data_ptr<float>();
+        set_strides(n.fs_stride, ds);
+      }
+      n.batch = p.batch;
+      n.seqlen = p.seqlen;
+      n.num_heads = p.num_heads;
+      n.num_heads_k = p.num_heads_k;
+      n.head_dim = p.head_dim;
+      n.scale = p.scale;
+      n.dtype = p.dtype;
+      const int status = linear_backward(n, tq, tk, g, want_init, stream, &r);
+      TORCH_CHECK(status == FA_OK, "fa_linear_bwd: status ", status);
+    }
+    return once({r.dq, r.dk, r.dv, r.ds}, grads);
+  }
+};
+
+// linear_dense_fwd(q, k, v, log_decay, scale, initial_state, want_final, with_grad, device,
+//                  stream) -> (out, final_state or None) | status | None
 PyObject* linear_dense_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Call c;
     fa_linear_args p = {};
-    if (n != 9 || !call_of(a[7], a[8], &c)) return none();
-    const at::Tensor* q = plain(a[0], c, 4);
-    if (!linear_dense(q, plain(a[1], c, 4), plain(a[2], c, 4), a[3], a[4], c, &p) ||
+    if (n != 10 || !call_of(a[8], a[9], &c)) return none();
+    const at::Tensor *q = plain(a[0], c, 4), *k = plain(a[1], c, 4), *v = plain(a[2], c, 4);
+    if (!linear_dense(q, k, v, a[3], a[4], c, &p) ||
         !state_of(a[5], *q, c, &p.initial_state, p.is_stride))
       return none();
-    const bool want_final = a[6] == Py_True;
+    const bool want_final = a[6] == Py_True, with_grad = a[7] == Py_True;
+    const at::Tensor decay = or_undefined(a[3]), init = or_undefined(a[5]);
     at::Tensor out, fin;
     int status;
     {
@@ -724,6 +951,23 @@ PyObject* linear_dense_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
       at::Tensor ws;
       if (bytes) ws = at::empty({(int64_t)bytes}, out.options().dtype(at::kByte));
       status = lib.linear_fwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, c.stream);
+      if (status == FA_OK && with_grad) {
+        auto node = std::shared_ptr<LinearNode>(new LinearNode(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(*q, *k, *v, init));
+        node->stream = c.stream;
+        node->p = p;
+        using torch::autograd::SavedVariable;
+        node->q = SavedVariable(*q, false);
+        node->k = SavedVariable(*k, false);
+        node->v = SavedVariable(*v, false);
+        node->decay = SavedVariable(decay, false);
+        if ((node->has_init = init.defined())) {
+          node->init = SavedVariable(init, false);
+          node->want_init = init.requires_grad();
+        }
+        torch::autograd::set_history(out, node);
+        if (want_final) torch::autograd::set_history(fin, node);
+      }
     }
     if (status != FA_OK) return PyLong_FromLong(status);
     PyObject* f = want_final ? THPVariable_Wrap(fin) : (Py_INCREF(Py_None), Py_None);
@@ -747,36 +991,16 @@ PyObject* linear_dense_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !state_of(a[7], *q, c, &p.d_final_state, p.fs_stride))
       return none();
     const bool want = a[8] == Py_True;
-    at::Tensor dq, dk, dv, ds;
+    LinearGrads r;
     int status;
     {
       NoGil no_gil;
-      dq = at::empty(q->sizes(), q->options().requires_grad(false));
-      dk = at::empty(k->sizes(), dq.options());
-      dv = at::empty(k->sizes(), dq.options());
-      p.dout = g->data_ptr();
-      p.dq = dq.data_ptr();
-      p.dk = dk.data_ptr();
-      p.dv = dv.data_ptr();
-      set_strides(p.do_stride, *g);
-      set_strides(p.dq_stride, dq);
-      set_strides(p.dk_stride, dk);
-      set_strides(p.dv_stride, dv);
-      if (want) {
-        ds = at::empty({q->size(0), q->size(2), q->size(3), q->size(3)},
-                       dq.options().dtype(at::kFloat));
-        p.d_initial_state = ds.data_ptr<float>();
-        set_strides(p.dis_stride, ds);
-      }
-      const size_t bytes = lib.linear_bwd_workspace(&p);
-      at::Tensor ws;
-      if (bytes) ws = at::empty({(int64_t)bytes}, dq.options().dtype(at::kByte));
-      status = lib.linear_bwd(&p, bytes ? ws.data_ptr() : nullptr, bytes, c.stream);
+      status = linear_backward(p, *q, *k, *g, want, c.stream, &r);
     }
     if (status != FA_OK) return PyLong_FromLong(status);
-    PyObject* d = want ? THPVariable_Wrap(ds) : (Py_INCREF(Py_None), Py_None);
-    return Py_BuildValue("NNNN", THPVariable_Wrap(dq), THPVariable_Wrap(dk), THPVariable_Wrap(dv),
-                         d);
+    PyObject* d = want ? THPVariable_Wrap(r.ds) : (Py_INCREF(Py_None), Py_None);
+    return Py_BuildValue("NNNN", THPVariable_Wrap(r.dq), THPVariable_Wrap(r.dk),
+                         THPVariable_Wrap(r.dv), d);
   });
 }
 
@@ -854,6 +1078,22 @@ PyObject* linear_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// foreign_leaf(tensor) -> bool: a leaf whose gradient accumulator a graph made on
+// another stream keeps alive.  The engine records an event on that stream when the
+// backward ends, which a stream capture does not survive (the process ends).
+PyObject* foreign_leaf(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 1 || !THPVariable_Check(a[0])) Py_RETURN_FALSE;
+    const at::Tensor& t = THPVariable_Unpack(a[0]);
+    if (!t.defined() || !t.is_cuda() || !t.requires_grad() || !t.is_leaf()) Py_RETURN_FALSE;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node || !node->stream()) Py_RETURN_FALSE;
+    const c10::impl::VirtualGuardImpl guard(c10::DeviceType::CUDA);
+    if (*node->stream() != guard.getStream(t.device())) Py_RETURN_TRUE;
+    Py_RETURN_FALSE;
+  });
+}
+
 // bind(...): the library's entry points, as addresses, in the order of Entries.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   constexpr int kEntries = 16;
@@ -903,6 +1143,7 @@ PyMethodDef methods[] = {method<bind>("bind"),
                          method<linear_dense_bwd>("linear_dense_bwd"),
                          method<linear_prefill>("linear_prefill"),
                          method<linear_decode>("linear_decode"),
+                         method<foreign_leaf>("foreign_leaf"),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_fa_torch", nullptr, -1, methods};

@@ -125,7 +125,7 @@ def _launch_fwd(a, device):
 # ------------------------------------------------------------------ training
 
 def _forward(q, k, v, log_decay, scale, initial_state, want_final):
-    done = _native.linear_dense_fwd(q, k, v, log_decay, scale, initial_state, want_final)
+    done = _native.linear_dense_fwd(q, k, v, log_decay, scale, initial_state, want_final, False)
     if done is not None:
         return done
     H, Hk, D = _check_qkv(q, k, v, ("batch", "seqlen", "heads", "head_dim"))
@@ -205,7 +205,8 @@ def _backward(q, k, v, dout, log_decay, scale, initial_state, d_final, want_d_in
 
 
 class LinearAttnFunc(torch.autograd.Function):
-    """linear_attn_func under autograd: saves its inputs alone."""
+    """linear_attn_func under autograd, where the native node does not take the call:
+    saves its inputs alone."""
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, scale, initial_state, want_final):
@@ -253,6 +254,11 @@ def linear_attn_func(q, k, v, log_decay, scale=None, initial_state=None,
                                        for t in (q, k, v, log_decay, initial_state)):
         if isinstance(log_decay, torch.Tensor) and log_decay.requires_grad:
             raise ValueError("log_decay gets no gradient: pass log_decay.detach()")
+        _native.refuse_foreign_leaves({"q": q, "k": k, "v": v, "initial_state": initial_state})
+        done = _native.linear_dense_fwd(q, k, v, log_decay, scale, initial_state,
+                                        bool(return_final_state), True)
+        if done is not None:
+            return done if return_final_state else done[0]
         return LinearAttnFunc.apply(q, k, v, log_decay, scale, initial_state,
                                     bool(return_final_state))
     out, final = _forward(q, k, v, log_decay, scale, initial_state, bool(return_final_state))

@@ -80,6 +80,22 @@ def _run(name, what, first, args):
     return r
 
 
+def refuse_foreign_leaves(named):
+    """While the current stream is captured: RuntimeError where one of the tensors is a
+    leaf that a live autograd graph of another stream holds.  Its captured backward
+    would make the engine use that stream too, which ends the process."""
+    first = next(iter(named.values()))
+    if _missing or not (isinstance(first, torch.Tensor) and first.is_cuda) or \
+            not torch.cuda.is_current_stream_capturing():
+        return
+    module = _module or _extension()
+    for name, t in named.items():
+        if module is not None and module.foreign_leaf(t):
+            raise RuntimeError(f"{name} is a leaf of a live autograd graph made outside this "
+                               "capture; release that graph first, or capture with "
+                               f"{name}.detach().requires_grad_()")
+
+
 def dense_forward(q, k, v, scale, causal, window, with_lse):
     """(out, lse or None), or None."""
     if type(window) is not tuple or len(window) != 2:

@@ -181,8 +181,9 @@ def _backward(q, k, dq_out, dk_out, cos, sin, q_weight, k_weight, positions, eps
 
 
 class QkNormRopeFunc(torch.autograd.Function):
-    """qk_norm_rope under autograd: saves its inputs alone (q and k only where
-    they are normed; a rotation's gradient needs neither)."""
+    """qk_norm_rope under autograd, where the native node does not take the call: saves
+    its inputs alone (q and k only where they are normed; a rotation's gradient needs
+    neither)."""
 
     @staticmethod
     def forward(ctx, q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved):
@@ -209,7 +210,8 @@ class QkNormRopeFunc(torch.autograd.Function):
 
 
 def _norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved):
-    done = _native.norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved)
+    done = _native.norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved,
+                             False)
     if done is not None:
         return done
     _check_heads(q, k, (3, 4))
@@ -245,6 +247,12 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, positions=None, e
     """
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
                                        for t in (q, k, q_weight, k_weight)):
+        _native.refuse_foreign_leaves({"q": q, "k": k, "q_weight": q_weight,
+                                       "k_weight": k_weight})
+        done = _native.norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved,
+                                 True)
+        if done is not None:
+            return done
         return QkNormRopeFunc.apply(q, k, cos, sin, q_weight, k_weight, positions, eps,
                                     interleaved)
     return _norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved)
