@@ -351,6 +351,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(Params p) {
   const int D = 8 * p.chunks;
   for (int i = threadIdx.x; i < D; i += kThreads) {
     float s = 0.f;
+#pragma unroll 8
     for (int g = 0; g < G; ++g) s += sums[g][i];
     p.partial[(int64_t)blockIdx.x * D + i] = s;
   }
@@ -369,12 +370,15 @@ __global__ __launch_bounds__(1024) void weight_grad_kernel(const float* partial,
   const int n = is_q ? nq : nk;
   const int col = blockIdx.x * 16 + threadIdx.x % 16, part = threadIdx.x / 16;
   float s = 0.f;
-  if (col < D)
+  if (col < D) {
+#pragma unroll 8
     for (int i = part; i < n; i += 64) s += src[(int64_t)i * D + col];
+  }
   sums[part][threadIdx.x % 16] = s;
   __syncthreads();
   if (part != 0 || col >= D) return;
   s = 0.f;
+#pragma unroll
   for (int i = 0; i < 64; ++i) s += sums[i][threadIdx.x];
   if (f32)
     static_cast<float*>(out)[col] = s;
