@@ -318,11 +318,16 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
   constexpr int NT = kTerms<T>;
   // Whether 128 or more registers hold what a chunk does not change.
   constexpr bool kKeep = D < 256;
-  __shared__ __align__(16) char lds_q[STATE_ONLY ? 16 : Tile::kBytes];
-  __shared__ __align__(16) char lds_k[Tile::kBytes];
-  __shared__ __align__(16) char lds_v[Tile::kBytes];
+  // Buffers of a chunk's rows: with two, the next chunk's rows go to LDS while this
+  // one is worked on, and one barrier of three goes: [2, 8192, 16, 128] forward 119 ->
+  // 108 us.  head_dim 256 has no LDS for it; at 64 a third workgroup on the CU is
+  // worth more ([4, 2048, 16, 64] backward 54 us, 62 us with two buffers).
+  constexpr int NB = D == 128 ? 2 : 1;
+  __shared__ __align__(16) char lds_q[STATE_ONLY ? 16 : NB * Tile::kBytes];
+  __shared__ __align__(16) char lds_k[NB * Tile::kBytes];
+  __shared__ __align__(16) char lds_v[NB * Tile::kBytes];
   __shared__ __align__(16) char lds_p[STATE_ONLY ? 16 : Scores::kBytes];
-  __shared__ __align__(16) float weight[kChunk];  // of row j in the state's update
+  __shared__ __align__(16) float weight[NB * kChunk];  // of row j in the state's update
   __shared__ float powers[STATE_ONLY ? 1 : kChunk + 17];
 
   const int h = blockIdx.x % p.heads, slot = blockIdx.x / p.heads;
@@ -412,8 +417,7 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
   }
 
   const int op_at = Tile::at(lc) + 16 * lq;  // operand reads of Q and K rows
-  const char* kt_p = lds_k + transposed_at<Tile>();
-  const char* vt_p = lds_v + transposed_at<Tile>() + 32 * wave;
+  const int tr_at = transposed_at<Tile>();   // transposing reads of K and V rows
   const int p_at = Scores::at(lc);
 
   // The two tiles above the diagonal that O's 32-key steps take in.
@@ -424,8 +428,7 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
           u32x2{0, 0});
   }
 
-  int weights_n = 0;  // rows of the chunk that `weight` and dm1 (l^n - 1) are for
-  float dm1 = 0.f;
+  float dm1 = 0.f;  // l^n - 1 for the chunk's n rows
   int held = 0;       // S is held times 2^held (fp16)
   const float p_scale = a.p_scale, inter_scale = a.inter_scale;
   auto p_factor = [&](int tile, int i) {
@@ -446,49 +449,70 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
   // |weight| < 2^weight_top (upd_scale 0 or not finite: no scaling to speak of)
   const int weight_top = min(max(exponent(a.upd_scale), -60), 60) + 1;
 
-  // The rows of O that the last chunk left in V's place, 16 bytes x 2 a thread (at
-  // the places where the thread puts its part of the next V).
-  auto write_rows = [&](int c, int n, int tid) {
+  // The rows of O that chunk c left in V's place, 16 bytes x 2 a thread (at the
+  // places where the thread puts its part of a later V).
+  auto write_rows = [&](int c, int buf, int tid) {
+    const int n = min(kChunk, nrows - c);
     const rsrc_t rs = make_rsrc(static_cast<uint16_t*>(a.out) + batch * a.os[0] +
                                     lowest(c, n) * a.os[1] + h * a.os[2],
                                 (uint32_t)((n - 1) * a.os[1] + D) * 2u);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
       __builtin_amdgcn_raw_buffer_store_b128(
-          ld16(lds_v + place_of<D>(tid) + u * Tile::at(L::RPT)), rs,
+          ld16(lds_v + buf * Tile::kBytes + place_of<D>(tid) + u * Tile::at(L::RPT)), rs,
           row_offset(L::RPT * u + tid / L::CPR, n, step, 2 * (uint32_t)a.os[1],
                      16 * (tid % L::CPR)),
           0, 0);
   };
+  // Chunk c's rows, which have been loaded, and its weights into a buffer.
+  auto stage = [&](int c, int buf, int tid) {
+    if (!STATE_ONLY) store_grouped<D>(sq, lds_q + buf * Tile::kBytes, tid);
+    store_rows<D>(sk, lds_k + buf * Tile::kBytes, tid);
+    store_rows<D>(sv, lds_v + buf * Tile::kBytes, tid);
+    // Rows at or behind n are zeros: their weight only has to be finite.
+    const int n = min(kChunk, nrows - c);
+    if (tid < kChunk)
+      weight[buf * kChunk + tid] = a.upd_scale * fast_exp2(g2 * (float)max(n - 1 - tid + sh, 0));
+  };
+  const bool out16 = !STATE_ONLY && !a.out_f32;
+  if constexpr (NB == 2) {
+    stage(0, 0, threadIdx.x);
+    if (kChunk < nrows) load_chunk(kChunk, threadIdx.x);
+    __syncthreads();
+  }
 
   for (int c = 0; c < nrows; c += kChunk) {
     const int n = min(kChunk, nrows - c);
+    const int buf = NB == 2 ? c / kChunk & 1 : 0;
     // At head_dim 256 addresses are formed anew in every chunk: kept, they are the
     // registers that no longer fit, and a reload from scratch waits for the rows on
     // their way.
     int tid = threadIdx.x;
     if constexpr (!kKeep) asm volatile("" : "+v"(tid));
-    __syncthreads();  // the last chunk's LDS reads are done, and its O is there
-    if constexpr (!STATE_ONLY) {
-      if (c > 0 && !a.out_f32) write_rows(c - kChunk, kChunk, tid);
-      store_grouped<D>(sq, lds_q, tid);
+    if constexpr (NB == 1) {
+      __syncthreads();  // the last chunk's LDS reads are done, and its O is there
+      if (out16 && c > 0) write_rows(c - kChunk, 0, tid);
+      stage(c, 0, tid);
+      __syncthreads();
+      if (c + kChunk < nrows) load_chunk(c + kChunk, tid);
     }
-    store_rows<D>(sk, lds_k, tid);
-    store_rows<D>(sv, lds_v, tid);
-    if (n != weights_n) {
-      // Rows at or behind n are zeros: their weight only has to be finite.
-      if (threadIdx.x < kChunk)
-        weight[threadIdx.x] =
-            a.upd_scale * fast_exp2(g2 * (float)max(n - 1 - (int)threadIdx.x + sh, 0));
-      weights_n = n;
-      dm1 = expm1f(g * (float)n);
-    }
-    __syncthreads();
-    if (c + kChunk < nrows) load_chunk(c + kChunk, tid);
+    // The next chunk into the other buffer, whose readers were done before the last
+    // barrier, and the last chunk's O out of it.
+    auto turn_over = [&]() {
+      if constexpr (NB == 2) {
+        if (out16 && c > 0) write_rows(c - kChunk, buf ^ 1, tid);
+        if (c + kChunk < nrows) stage(c + kChunk, buf ^ 1, tid);
+        if (c + 2 * kChunk < nrows) load_chunk(c + 2 * kChunk, tid);
+      }
+    };
+    if (c == 0 || n < kChunk) dm1 = expm1f(g * (float)n);
+    const char* q_rows = lds_q + buf * Tile::kBytes;
+    const char* k_rows = lds_k + buf * Tile::kBytes;
+    char* v_rows = lds_v + buf * Tile::kBytes;
 
     u32x4 vt[kChunk / 32];  // the wave's columns of V, for O and for the update
 #pragma unroll
-    for (int s = 0; s < kChunk / 32; ++s) vt[s] = read_transposed<Tile>(vt_p, s);
+    for (int s = 0; s < kChunk / 32; ++s) vt[s] = read_transposed<Tile>(v_rows + tr_at + 32 * wave, s);
     f32x4 o[4];
     if constexpr (!STATE_ONLY) {
       // P^T = K Q^T with the decay, rounded, as P's rows in LDS.
@@ -497,8 +521,8 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
         const int tile = wave + L::NW * np;
         if (tile < 10) {
           const int it = (tile >= 1) + (tile >= 3) + (tile >= 6), jt = tile - it * (it + 1) / 2;
-          const char* kq = lds_k + Tile::at(16 * jt + lc) + 8 * lq;
-          const char* qq = lds_q + op_at + it * Tile::at(16);
+          const char* kq = k_rows + Tile::at(16 * jt + lc) + 8 * lq;
+          const char* qq = q_rows + op_at + it * Tile::at(16);
           f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int kk = 0; kk < D / 32; ++kk) {
@@ -536,7 +560,7 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
           sf[i] = T::pack(S[dt + i / 2][2 * (i & 1)] * down, S[dt + i / 2][2 * (i & 1) + 1] * down);
 #pragma unroll
         for (int it = 0; it < 4; ++it)
-          o[it] = T::mma16(sf, ld16(lds_q + op_at + it * Tile::at(16) + 32 * dt), o[it]);
+          o[it] = T::mma16(sf, ld16(q_rows + op_at + it * Tile::at(16) + 32 * dt), o[it]);
       }
 #pragma unroll
       for (int it = 0; it < 4; ++it) o[it] *= up * (kKeep ? rowf[it] : row_factor(it));
@@ -544,6 +568,7 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
 
     auto finish = [&]() {
       __syncthreads();  // P is there
+      turn_over();
       // O^T += V^T P^T
 #pragma unroll
       for (int s = 0; s < kChunk / 32; ++s)
@@ -564,7 +589,7 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
         // Into V's columns of this wave, which no other wave reads.
 #pragma unroll
         for (int it = 0; it < 4; ++it)
-          st8(lds_v + Tile::at(16 * it + lc) + 32 * wave + 8 * lq,
+          st8(v_rows + Tile::at(16 * it + lc) + 32 * wave + 8 * lq,
               u32x2{T::pack(o[it][0], o[it][1]), T::pack(o[it][2], o[it][3])});
       }
     };
@@ -591,8 +616,8 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
 #pragma unroll
       for (int s = 0; s < kChunk / 32; ++s) {
         float x[8];
-        const f32x4 w0 = *reinterpret_cast<const f32x4*>(weight + 32 * s + 4 * lq) * hold;
-        const f32x4 w1 = *reinterpret_cast<const f32x4*>(weight + 32 * s + 16 + 4 * lq) * hold;
+        const f32x4 w0 = *reinterpret_cast<const f32x4*>(weight + buf * kChunk + 32 * s + 4 * lq) * hold;
+        const f32x4 w1 = *reinterpret_cast<const f32x4*>(weight + buf * kChunk + 32 * s + 16 + 4 * lq) * hold;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           x[2 * i] = T::lo(vt[s][i]) * (i < 2 ? w0[2 * i] : w1[2 * i - 4]);
@@ -602,7 +627,7 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
         split_terms<T, NT>(x, term);
 #pragma unroll
         for (int dt = 0; dt < L::DT; ++dt) {
-          const u32x4 kt = read_transposed<Tile>(kt_p + 32 * dt, s);
+          const u32x4 kt = read_transposed<Tile>(k_rows + tr_at + 32 * dt, s);
 #pragma unroll
           for (int t = 0; t < NT; ++t) S[dt] = T::mma16(kt, term[t], S[dt]);
         }
@@ -612,6 +637,7 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
     // that formed P's tiles are behind the others; at head_dim 256 there are no
     // registers to keep O through it.
     if constexpr (STATE_ONLY) {
+      turn_over();
       update();
     } else if constexpr (D < 256) {
       update();
@@ -620,6 +646,7 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
       finish();
       update();
     }
+    if constexpr (NB == 2) __syncthreads();  // the next chunk is there, and this one's O
   }
 
   const float out = pow2(-held);
@@ -629,10 +656,10 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
       *reinterpret_cast<f32x4*>(seg_state + state_image<D>(wave, dt, lane)) = S[dt] * out;
     return;
   }
-  if (!a.out_f32) {
+  if (out16) {
     __syncthreads();
     const int c = (nrows - 1) / kChunk * kChunk;
-    write_rows(c, nrows - c, threadIdx.x);
+    write_rows(c, NB == 2 ? c / kChunk & 1 : 0, threadIdx.x);
   }
   float* fin = sg.seg == sg.nseg - 1 ? fin_of(p, a, sg.b, h) : nullptr;
   if (fin) {
