@@ -485,7 +485,8 @@ int fa_norm_rope_and_cache(const fa_norm_rope_cache_args* args, void* stream);
 /* and keeps nothing; slots in use must be distinct.  prefix_kv_lens (NULL: */
 /* all start from the initial state): a sequence with prefix_kv_lens[b] <=  */
 /* 0 starts from zero.  A sequence of no tokens leaves its slot of          */
-/* final_state as it was.                                                   */
+/* final_state as it was.  out may be q (with its strides) and must not     */
+/* overlap k or v.                                                          */
 /* The arithmetic: matrix products of dtype operands with fp32 sums; the    */
 /* states and every sum are fp32.                                           */
 /* ------------------------------------------------------------------------ */

@@ -404,8 +404,9 @@ static int check_rope(const Args* a, const char* who, int64_t tokens, int heads_
                 who);
   if (!aligned16(a->q_weight) || !aligned16(a->k_weight))
     return fail(FA_E_UNSUPPORTED, "%s: weights must be 16-byte aligned", who);
-  // Rows are counted in 31 bits on the device.
-  if (tokens > kIntMax / (a->num_heads > heads_k ? a->num_heads : heads_k))
+  // Rows are counted in 31 bits on the device, and a launch has at most 2^32 - 1
+  // threads: up to 32 a row of q, k and v.
+  if (tokens > kIntMax / 16 / ((int64_t)a->num_heads + 2 * heads_k))
     return fail(FA_E_UNSUPPORTED, "%s: problem too large", who);
   return ok();
 }
@@ -535,10 +536,11 @@ static int check_row_strides(const char* who, std::initializer_list<const int64_
   return ok();
 }
 
-// Workgroups of one launch: sequences x heads x up to 64 parts of a state, and
-// the segments.
+// Threads of one launch, at most 2^32 - 1: 256 for each of up to 64 parts of every
+// (sequence, head)'s state, and 4 D for each segment.
 static int check_linear_grid(const char* who, int64_t batch, int heads, int D, int64_t groups) {
-  if (batch * heads > kIntMax / (D * D / 1024) || groups > kIntMax)
+  const int64_t most = 2 * kIntMax;
+  if (batch * heads > most / 256 / (D * D / 1024) || groups > most / (4 * D))
     return fail(FA_E_UNSUPPORTED, "%s: problem too large", who);
   return ok();
 }
@@ -599,8 +601,9 @@ static int check_linear_bwd(const fa_linear_bwd_args* a) {
   if ((st = check_state(who, a->initial_state, a->is_stride)) != FA_OK) return st;
   if ((st = check_state(who, a->d_final_state, a->fs_stride)) != FA_OK) return st;
   if ((st = check_state(who, a->d_initial_state, a->dis_stride)) != FA_OK) return st;
+  // (Shared heads: a thread for each 8 components of dk and of dv.)
   if (a->seqlen > kIntMax / 2 ||
-      (int64_t)a->batch * a->seqlen > (int64_t)kIntMax * 4 / a->num_heads_k)
+      (int64_t)a->batch * a->seqlen > 2 * kIntMax / (a->head_dim / 8) / a->num_heads_k)
     return fail(FA_E_UNSUPPORTED, "%s: problem too large", who);
   return check_linear_grid(who, a->batch, a->num_heads, a->head_dim,
                            a->batch && a->seqlen ? fa::linear_bwd_workgroups(*a) : 0);

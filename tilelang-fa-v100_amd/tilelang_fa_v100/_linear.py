@@ -292,7 +292,7 @@ def linear_attn_prefill(q, k, v, log_decay, state, query_start_loc, prefix_kv_le
         state_indices: [B] integers, each sequence's slot, distinct; None:
             0 .. B - 1.  A sequence whose slot is not in the pool (negative:
             padding) starts from zeros and keeps no state.
-        out: written in place when given.
+        out: written in place when given; may be q, must not overlap k or v.
     Returns:
         out [T, H, D].  Rows of no sequence are not written, and a sequence of
         no tokens leaves its slot as it was.  No gradients.
