@@ -612,7 +612,8 @@ at::Tensor or_undefined(PyObject* o) {
 
 // norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved, with_grad,
 //           device, stream) -> (q_out, k_out) | status | None.  Positions: None or a vector.
-// with_grad: the outputs have a node in the autograd graph.
+// with_grad True: the outputs have a node in the autograd graph; None: a call that
+// would need one is handed back.
 PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Call c;
@@ -624,6 +625,9 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !rope_sizes(*q, *k, a[6], c, &p))
       return none();
     const bool with_grad = a[9] == Py_True;
+    if (a[9] == Py_None && at::GradMode::is_enabled())
+      for (int i : {0, 1, 4, 5})
+        if (a[i] != Py_None && THPVariable_Unpack(a[i]).requires_grad()) return none();
     const at::Tensor cos = or_undefined(a[2]), sin = or_undefined(a[3]), qw = or_undefined(a[4]),
                      kw = or_undefined(a[5]), pos = or_undefined(a[6]);
     at::Tensor q_out, k_out;

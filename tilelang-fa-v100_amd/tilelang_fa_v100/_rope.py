@@ -245,6 +245,10 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, positions=None, e
         (q_out, k_out), new contiguous tensors.  Differentiable with respect to
         q, k and the weights.  Computed in fp32, rounded once.
     """
+    done = _native.norm_rope(q, k, cos, sin, q_weight, k_weight, positions, eps, interleaved,
+                             None)
+    if done is not None:
+        return done
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
                                        for t in (q, k, q_weight, k_weight)):
         _native.refuse_foreign_leaves({"q": q, "k": k, "q_weight": q_weight,
