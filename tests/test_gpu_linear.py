@@ -432,3 +432,25 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         got, got_s = tok_out.clone(), state.clone()
         assert torch.equal(fa.linear_attn_decode(*tok, g, mine), got) and torch.equal(mine, got_s)
+
+
+# One or two heads want more segments than the main launch adds up: their states
+# are joined before it.
+JOINED = [
+    (1, 2053, 1, 1, 128, torch.float16, True, "mixed"),
+    (2, 1300, 2, 1, 64, torch.bfloat16, True, "mixed"),
+    (1, 2500, 2, 2, 64, torch.float16, False, "none"),
+]
+
+
+@pytest.mark.parametrize("case", JOINED, ids=[f"S{c[1]}_H{c[2]}_{c[3]}_D{c[4]}" for c in JOINED])
+def test_many_segments(case):
+    test_forward_matches_reference(case)
+    test_gradients_match_reference(case)
+
+
+@pytest.mark.parametrize("lens", [(9000, 0, 5003, 1, 2380), (16384,), (64,) * 40 + (3000, 1)],
+                         ids=["long", "one", "many"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_packed_segments(lens, D):
+    test_prefill_matches_reference(lens, 2, 1, D, torch.bfloat16)

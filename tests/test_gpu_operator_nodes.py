@@ -59,7 +59,7 @@ def test_native_and_python_gradients_are_the_same_bits(name, monkeypatch):
 
 @pytest.mark.parametrize("name", CALLS)
 def test_partial_and_odd_gradients(name, path):
-    """One output's gradient alone, expanded, in fp32-free types; some of the leaves."""
+    """One output's gradient alone, expanded or misaligned; some of the leaves."""
     call, leaves, _ = CALLS[name]()
     out = call()
     want = torch.autograd.grad(out, leaves, [torch.ones_like(out[0])]

@@ -17,10 +17,19 @@
 //
 // Work split: a workgroup holds one (sequence, head, segment)'s state in
 // registers and walks its chunks; each wave owns 16 of the state's columns (D / 16
-// waves, 128 registers each: at head_dim 128 two workgroups and 16 waves on a CU).  Where sequences x heads are too few for the GPU, sequences are cut
-// into segments: one launch forms every segment's own state, and the main launch
-// starts each segment from the states of those before it, which it adds up itself
-// (few segments) or finds joined by linear_scan_kernel.
+// waves).  On a CU: three workgroups at head_dim 64 (registers, 41 KB of LDS), one at
+// 128 (two LDS buffers, 122 KB) and one at 256 (16 waves of 128 registers).  Where
+// sequences x heads are too few for the GPU, sequences are cut into segments: one
+// launch forms every segment's own state, and the main launch starts each segment
+// from the states of those before it, which it adds up itself (few segments) or finds
+// joined by linear_scan_kernel.
+//
+// What bounds it: the chunks of a workgroup follow each other, and a chunk's phases
+// (operand reads, products, the split, barriers) hardly overlap.  At head_dim 128 a
+// chunk takes 3.4 us with 64 workgroups and 4.7 with 256 (long sequences, 3.6 TB/s);
+// of its 8416 cycles LDS is busy 49%, the matrix cores 29%, and the waves wait 41%.
+// [4, 2048, 16, 128] bf16: forward 43 us after 23 us for the segments' states,
+// the three gradients 128 us.
 //
 // Registers and LDS: the state's accumulators (row d in the registers, column e
 // in the lane) are, rounded, the A operand of O^T = S^T Q^T as they stand: S never
@@ -31,11 +40,11 @@
 // type, once each, as the attention kernels round P.  The state itself is fp32,
 // and its update is kept exact to it: l^{n-1-j} v_j is split into NT terms of the
 // input type whose products with k are exact (three of bf16's 8 bits or two of
-// fp16's 11 make up fp32's 24; two of bf16's, where no state is returned, were 2%
-// faster at head_dim 128, and outputs would then differ with what is asked for).
-// fp16's terms would leave its range below 2^-14:
-// there a wave holds its columns of S times a power of two that keeps the largest
-// weighted value near 2^13, and takes it out at every use.
+// fp16's 11 make up fp32's 24; two of bf16's, where no state is returned, would save
+// 8% at head_dim 128 (115 -> 105 us in one segment), and outputs would then differ with
+// what is asked for).  fp16's terms would leave its range below 2^-14: there a wave
+// holds its columns of S times a power of two that keeps the largest weighted value
+// near 2^13, and takes it out at every use.
 #include "fa_common.h"
 #include "fa_fwd_d128.h"
 #include "fa_internal.h"
@@ -83,9 +92,12 @@ struct LinParams {
 // states of those before it, which the main kernel adds up; or linear_scan_kernel
 // has put it into its slot.
 enum { kWhole = 0, kAdded = 1, kScanned = 2 };
-// Segments of a sequence that are added up (none at head_dim 256, whose kernel has
-// no registers for it).
-constexpr int max_added(int D) { return D < 256 ? 8 : 1; }
+// Segments up to which they are added up (none at head_dim 256, whose kernel has no
+// registers for it).  One sequence: [2, 8192, 8, 64] in 16 takes 38 us added and 41
+// joined, [1, 16384, 4, 128] in 32 takes 68 and 63.  Packed sequences share the count,
+// which bounds each one's: eight of 600 to 4096 rows, 16 heads, head_dim 128, in 18
+// take 167 and 175 us; one of 17000 among single tokens, in 34, 194 and 196.
+constexpr int max_added(int D, bool shared) { return D == 256 ? 1 : (shared ? 32 : 16); }
 
 struct Segment {
   int b, seg, nseg;  // sequence, segment, segments of the sequence; b < 0: none
@@ -241,8 +253,8 @@ __device__ __forceinline__ void store_rows(const Staged& s, char* lds, int tid) 
 }
 
 // Operand with row or column lane % 16 and k = 32 s + 4 (lane / 16) + 0..3 and the
-// same + 16, from 16 columns of a row-major [k][column] tile in LDS; p: the tile, transposed_at of the
-// lane, and the 16 columns' place.
+// same + 16, from 16 columns of a row-major [k][column] tile in LDS; p: the tile,
+// transposed_at of the lane, and the 16 columns' place.
 template <class Tile>
 __device__ __forceinline__ u32x4 read_transposed(const char* p, int s) {
   const u32x2 lo = lds_read_tr(p + s * Tile::at(32));
@@ -316,7 +328,8 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
   using Tile = typename L::Tile;
   using Scores = typename L::Scores;
   constexpr int NT = kTerms<T>;
-  // Whether 128 or more registers hold what a chunk does not change.
+  // Whether registers hold what a chunk does not change (head_dim 256 has 128 of them
+  // for a wave, and spills 23 to 39 as it is).
   constexpr bool kKeep = D < 256;
   // Buffers of a chunk's rows: with two, the next chunk's rows go to LDS while this
   // one is worked on, and one barrier of three goes: [2, 8192, 16, 128] forward 119 ->
@@ -387,18 +400,18 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
       }
       // The states of the segments before, in order.
       if constexpr (kKeep) {
-      const float decay = expm1f(g * (float)p.seglen);
-      const int64_t next = (int64_t)p.heads * D * D;
-      for (int s = sg.seg; s > 0; --s) {
-        const float* u = seg_state - s * next + state_image<D>(wave, 0, lane);
-        f32x4 x[L::DT];
+        const float decay = expm1f(g * (float)p.seglen);
+        const int64_t next = (int64_t)p.heads * D * D;
+        for (int s = sg.seg; s > 0; --s) {
+          const float* u = seg_state - s * next + state_image<D>(wave, 0, lane);
+          f32x4 x[L::DT];
 #pragma unroll
-        for (int dt = 0; dt < L::DT; ++dt) x[dt] = *reinterpret_cast<const f32x4*>(u + 256 * dt);
+          for (int dt = 0; dt < L::DT; ++dt) x[dt] = *reinterpret_cast<const f32x4*>(u + 256 * dt);
 #pragma unroll
-        for (int dt = 0; dt < L::DT; ++dt)
+          for (int dt = 0; dt < L::DT; ++dt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) S[dt][i] = fmaf(S[dt][i], decay, S[dt][i]) + x[dt][i];
-      }
+            for (int i = 0; i < 4; ++i) S[dt][i] = fmaf(S[dt][i], decay, S[dt][i]) + x[dt][i];
+        }
       }
     }
   }
@@ -616,8 +629,9 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
 #pragma unroll
       for (int s = 0; s < kChunk / 32; ++s) {
         float x[8];
-        const f32x4 w0 = *reinterpret_cast<const f32x4*>(weight + buf * kChunk + 32 * s + 4 * lq) * hold;
-        const f32x4 w1 = *reinterpret_cast<const f32x4*>(weight + buf * kChunk + 32 * s + 16 + 4 * lq) * hold;
+        const float* w = weight + buf * kChunk + 32 * s + 4 * lq;
+        const f32x4 w0 = *reinterpret_cast<const f32x4*>(w) * hold;
+        const f32x4 w1 = *reinterpret_cast<const f32x4*>(w + 16) * hold;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           x[2 * i] = T::lo(vt[s][i]) * (i < 2 ? w0[2 * i] : w1[2 * i - 4]);
@@ -672,7 +686,8 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
 
 // Joins the segments' states in order: each slot's own state becomes the state
 // before it.  A thread holds four components, in the workspace's layout
-// (state_image): rows d .. d + 3 of column e.
+// (state_image): rows d .. d + 3 of column e.  Bound by the states' memory: 9 us for
+// eight packed prompts of 16 heads at head_dim 128.
 template <int D>
 __global__ __launch_bounds__(256) void linear_scan_kernel(LinParams p) {
   constexpr int PARTS = D * D / 1024;
@@ -742,7 +757,8 @@ __global__ __launch_bounds__(256) void linear_group_sum_kernel(const float* part
 // One token for each sequence: the state is read, updated and written once.
 // Bound by that memory (8 D^2 bytes a sequence and head; D^2 * 5 flops).  A
 // workgroup takes COLS columns of one head's state: every load is issued before
-// the first use, and a column's sum over d stays inside the workgroup.
+// the first use, and a column's sum over d stays inside the workgroup.  64 x 32 states
+// at head_dim 128: 57 us, 4.7 TB/s (a large copy: 5.2); 4 x 16: 4.6 us.
 template <class T, int D, int COLS>
 __global__ __launch_bounds__(256) void linear_decode_kernel(fa_linear_decode_args a) {
   constexpr int LANES = COLS / 4, ROWS = 256 / LANES, N = D / ROWS, SLICES = D / COLS;
@@ -825,6 +841,7 @@ int segment_rows(int64_t tokens, int64_t units, int64_t seqs, int D) {
   const double lat = D == 64 ? 2.1 : (D == 128 ? 3.5 : 8.0);
   const double mem = D == 64 ? 1.8 : (D == 128 ? 3.6 : 7.2);
   const double bytes_us = 4.0 * D * D / 5e6;  // a state once through memory
+  const int added = max_added(D, seqs > 1);
   const int64_t chunks = (tokens + kChunk - 1) / kChunk;
   double best = 0;
   int64_t rows = chunks;
@@ -835,8 +852,7 @@ int segment_rows(int64_t tokens, int64_t units, int64_t seqs, int D) {
     double t = launch_us(units * segments, c, per_cu, lat, mem);
     if (n > 1)
       t += launch_us(units * (segments - seqs), c, 2 * per_cu, 0.6 * lat, 0.5 * mem) +
-           units * n * (n <= max_added(D) ? 1 + n / 2 : 4) * bytes_us +
-           (n <= max_added(D) ? 0 : 5);
+           units * n * (n <= added ? 1 + n / seqs / 2 : 4) * bytes_us + (n <= added ? 0 : 5);
     if (n == 1 || t < best) {
       best = t;
       rows = c;
@@ -849,9 +865,10 @@ int segment_rows(int64_t tokens, int64_t units, int64_t seqs, int D) {
 int64_t set_segments(LinParams& p, int D) {
   // (Packed: the sequences' lengths are on the device.)
   const int64_t units = (int64_t)p.heads * p.npass * (p.starts ? 1 : p.batch);
-  p.seglen = segment_rows(p.seqlen, units, p.starts ? p.batch : 1, D);
+  const int64_t seqs = p.starts ? p.batch : 1;
+  p.seglen = segment_rows(p.seqlen, units, seqs, D);
   const int64_t most = ((int64_t)p.seqlen + p.seglen - 1) / p.seglen;
-  p.join = most == 1 ? kWhole : (most <= max_added(D) ? kAdded : kScanned);
+  p.join = most == 1 ? kWhole : (most <= max_added(D, seqs > 1) ? kAdded : kScanned);
   if (p.starts) {
     p.nseg = p.seqlen / p.seglen + p.batch;
     return p.nseg;
@@ -966,15 +983,22 @@ size_t part_bytes(const fa_linear_bwd_args& a) {
 
 template <class T, int D>
 hipError_t launch_decode_cols(const fa_linear_decode_args& a, hipStream_t st) {
-  // The fewest columns of a workgroup (32) while that leaves CUs without one.
+  // Wide slices (512-byte rows) where they give every CU a workgroup, before that 32
+  // columns: 4 x 32 states at head_dim 128 take 4.6 us in 32 columns and 5.3 wide, 8 x 32
+  // take 8.1 and 7.0.  At head_dim 64 a whole state (4 x 16: 3.3 and 3.2 us, 64 x 32: 13.9
+  // and 11.8).
   constexpr int WIDE = D < 128 ? D : 128;
   const int64_t heads = (int64_t)a.batch * a.num_heads;
-  if (heads * (D / WIDE) >= device_cu_count())
-    hipLaunchKernelGGL((linear_decode_kernel<T, D, WIDE>), dim3((unsigned)(heads * (D / WIDE))),
-                       dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((linear_decode_kernel<T, D, 32>), dim3((unsigned)(heads * (D / 32))),
-                       dim3(256), 0, st, a);
+  auto run = [&](auto kernel, int cols) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(heads * (D / cols))), dim3(256), 0, st, a);
+  };
+  if constexpr (D > 64) {
+    if (heads * (D / WIDE) < device_cu_count()) {
+      run(linear_decode_kernel<T, D, 32>, 32);
+      return hipGetLastError();
+    }
+  }
+  run(linear_decode_kernel<T, D, WIDE>, WIDE);
   return hipGetLastError();
 }
 
