@@ -9,10 +9,11 @@
 //
 // The backward is the same operator three times:
 //   dq: (q, k, v) -> (dO, v, k), state transposed, time forward;
-//   dk: (v, dO, q) and dv: (k, q, dO), time reversed, where the carried state
+//   dv: (k, q, dO) and dk: (v, dO, q), time reversed, where the carried state
 //   has its decay taken already (a row sees l^i of it instead of l^{i+1}, and
 //   the update's weights are l^{n-j}); its last value of the dv pass is the
-//   gradient of the initial state.
+//   gradient of the initial state.  dk's state is dv's transposed: a segment of dk
+//   starts from dv's.
 // One kernel runs all of them ("passes"), in one launch.
 //
 // Work split: a workgroup holds one (sequence, head, segment)'s state in
@@ -80,7 +81,7 @@ struct LinParams {
   const int32_t* starts;  // packed form
   const int32_t* prefix;
   const int32_t* slots;
-  float* ws;  // [pass][slot][head][D][D]: the segments' states
+  float* ws;  // [pass][slot][head][D][D]: the segments' states (of two passes at most)
   int32_t batch, seqlen, heads, npass;
   int32_t nseg;    // dense: segments of a sequence; packed: slots in all
   int32_t seglen;  // rows of a segment, a multiple of kChunk
@@ -92,6 +93,8 @@ struct LinParams {
 // states of those before it, which the main kernel adds up; or linear_scan_kernel
 // has put it into its slot.
 enum { kWhole = 0, kAdded = 1, kScanned = 2 };
+// Passes: the forward alone, or dq, dv and dk, whose states are dv's transposed.
+constexpr int kTwin = 2;
 // Segments up to which they are added up (none at head_dim 256, whose kernel has no
 // registers for it).  One sequence: [2, 8192, 8, 64] in 16 takes 38 us added and 41
 // joined, [1, 16384, 4, 128] in 32 takes 68 and 63.  Packed sequences share the count,
@@ -320,6 +323,27 @@ __device__ __forceinline__ int state_image(int wave, int dt, int lane) {
   return ((wave * (D / 16) + dt) * 64 + lane) * 4;
 }
 
+// A wave's part of a segment's state; transposed: u is the state of the pass whose
+// states are this one's transposed.
+template <int D>
+__device__ __forceinline__ void load_state(f32x4 (&x)[D / 16], const float* u, int wave, int lane,
+                                           bool transposed) {
+  if (transposed) {
+    // Row 16 dt + 4 lq + i and column 16 wave + lc here are that column and row there.
+    const int quad = 16 * ((lane & 15) >> 2) + 4 * (lane >> 4);
+    const float* t = u + state_image<D>(0, wave, quad) + (lane & 3);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[dt][i] = t[state_image<D>(dt, 0, i)];
+  } else {
+    const float* t = u + state_image<D>(wave, 0, lane);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+      x[dt] = *reinterpret_cast<const f32x4*>(t + state_image<D>(0, dt, 0));
+  }
+}
+
 // One segment of one head.  STATE_ONLY: forms the segment's own state (from
 // zero) into the workspace and no output.
 template <class T, int D, bool STATE_ONLY>
@@ -380,16 +404,16 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
 
   // State column 16 wave + lc, rows 16 dt + 4 lq + (0..3).
   f32x4 S[L::DT];
+  const bool twin = blockIdx.y == kTwin;
+  const int64_t slots = (int64_t)p.nseg * (p.starts ? 1 : p.batch);
   float* seg_state =
-      p.ws + (((int64_t)blockIdx.y * p.nseg * (p.starts ? 1 : p.batch) + slot) * p.heads + h) * D * D;
+      p.ws + ((min((int)blockIdx.y, kTwin - 1) * slots + slot) * p.heads + h) * D * D;
   const int col = 16 * wave + lc;
 #pragma unroll
   for (int dt = 0; dt < L::DT; ++dt) S[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (!STATE_ONLY) {
     if (p.join == kScanned) {
-#pragma unroll
-      for (int dt = 0; dt < L::DT; ++dt)
-        S[dt] = *reinterpret_cast<const f32x4*>(seg_state + state_image<D>(wave, dt, lane));
+      load_state<D>(S, seg_state, wave, lane, twin);
     } else {
       if (const float* src = init_of(p, a, sg.b, h)) {
 #pragma unroll
@@ -403,10 +427,8 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
         const float decay = expm1f(g * (float)p.seglen);
         const int64_t next = (int64_t)p.heads * D * D;
         for (int s = sg.seg; s > 0; --s) {
-          const float* u = seg_state - s * next + state_image<D>(wave, 0, lane);
           f32x4 x[L::DT];
-#pragma unroll
-          for (int dt = 0; dt < L::DT; ++dt) x[dt] = *reinterpret_cast<const f32x4*>(u + 256 * dt);
+          load_state<D>(x, seg_state - s * next, wave, lane, twin);
 #pragma unroll
           for (int dt = 0; dt < L::DT; ++dt)
 #pragma unroll
@@ -819,11 +841,11 @@ __global__ __launch_bounds__(256) void linear_decode_kernel(fa_linear_decode_arg
 
 // Microseconds of a launch whose `groups` workgroups walk `chunks` chunks each,
 // `per_cu` of them on a CU at a time: a chunk takes `lat` for one workgroup alone
-// and `mem` for each of those on a CU where memory is the bound.
+// and `mem` for each of those on a CU.
 double launch_us(int64_t groups, int64_t chunks, int per_cu, double lat, double mem) {
   const int64_t cus = device_cu_count(), full = groups / (cus * per_cu);
   const int64_t rest = groups - full * cus * per_cu;
-  const double start = 4.0;
+  const double start = 4.5;
   double t = full * (start + chunks * std::max(lat, per_cu * mem));
   if (rest > 0) t += start + chunks * std::max(lat, (double)((rest + cus - 1) / cus) * mem);
   return t;
@@ -831,16 +853,19 @@ double launch_us(int64_t groups, int64_t chunks, int per_cu, double lat, double 
 
 // Rows of a segment.  More segments fill the GPU, and each costs a state formed
 // twice and carried through memory: the count with the least time by the model
-// above.  Its constants are MI355X measurements (us a chunk); it is within 15% of
-// the measured times of [4, 2048, 16, 128], [2, 8192, 16, 128] and one sequence of
-// 18688 rows at 1 to 32 segments, and picks the fastest or one within 5% of it.
-// tokens: of one sequence, or of all `seqs` packed ones, which end in a part of a
-// segment each.
-int segment_rows(int64_t tokens, int64_t units, int64_t seqs, int D) {
-  const int per_cu = D == 64 ? 3 : 1;
-  const double lat = D == 64 ? 2.1 : (D == 128 ? 3.5 : 8.0);
-  const double mem = D == 64 ? 1.8 : (D == 128 ? 3.6 : 7.2);
-  const double bytes_us = 4.0 * D * D / 5e6;  // a state once through memory
+// above.  Its constants (us a chunk, TB/s) are fitted to MI355X times of the forward
+// and the backward of 21 shapes, one to forty heads and 1024 to 32768 rows, at 1 to 64
+// segments: what it picks is within 3% of the fastest of them, 0.3% on average.
+// units: sequences x heads x passes; state_units: of those, the ones whose segments'
+// states are formed.  tokens: of one sequence, or of all `seqs` packed ones, which end
+// in a part of a segment each.
+int segment_rows(int64_t tokens, int64_t units, int64_t state_units, int64_t seqs, int D) {
+  const int per_cu = D == 64 ? 3 : 1, state_per_cu = D == 64 ? 6 : (D == 128 ? 2 : 1);
+  const double chunk = D == 64 ? 1.8 : (D == 128 ? 3.8 : 10.5);
+  const double state_lat = D == 64 ? 0.75 : (D == 128 ? 1.5 : 4.5);
+  const double state_mem = D == 64 ? 0.33 : state_lat;
+  // A state once through memory; smaller ones stay in the last cache.
+  const double bytes_us = 4.0 * D * D / (D < 256 ? 10e6 : 5e6);
   const int added = max_added(D, seqs > 1);
   const int64_t chunks = (tokens + kChunk - 1) / kChunk;
   double best = 0;
@@ -849,9 +874,9 @@ int segment_rows(int64_t tokens, int64_t units, int64_t seqs, int D) {
     const int64_t c = (chunks + n - 1) / n;
     if (n > 1 && (chunks + c - 1) / c < n) continue;  // the same as fewer
     const int64_t segments = std::max(n + (seqs - 1) / 2, seqs);
-    double t = launch_us(units * segments, c, per_cu, lat, mem);
+    double t = launch_us(units * segments, c, per_cu, chunk, chunk);
     if (n > 1)
-      t += launch_us(units * (segments - seqs), c, 2 * per_cu, 0.6 * lat, 0.5 * mem) +
+      t += launch_us(state_units * (segments - seqs), c, state_per_cu, state_lat, state_mem) +
            units * n * (n <= added ? 1 + n / seqs / 2 : 4) * bytes_us + (n <= added ? 0 : 5);
     if (n == 1 || t < best) {
       best = t;
@@ -861,12 +886,15 @@ int segment_rows(int64_t tokens, int64_t units, int64_t seqs, int D) {
   return (int)(rows * kChunk);
 }
 
+// Passes whose segments' states are formed.
+int state_passes(const LinParams& p) { return std::min<int>(p.npass, kTwin); }
+
 // Cuts p's sequences; returns the slots in all.
 int64_t set_segments(LinParams& p, int D) {
   // (Packed: the sequences' lengths are on the device.)
   const int64_t units = (int64_t)p.heads * p.npass * (p.starts ? 1 : p.batch);
   const int64_t seqs = p.starts ? p.batch : 1;
-  p.seglen = segment_rows(p.seqlen, units, seqs, D);
+  p.seglen = segment_rows(p.seqlen, units, units / p.npass * state_passes(p), seqs, D);
   const int64_t most = ((int64_t)p.seqlen + p.seglen - 1) / p.seglen;
   p.join = most == 1 ? kWhole : (most <= max_added(D, seqs > 1) ? kAdded : kScanned);
   if (p.starts) {
@@ -878,18 +906,18 @@ int64_t set_segments(LinParams& p, int D) {
 }
 
 size_t state_bytes(const LinParams& p, int64_t slots, int D) {
-  return p.join != kWhole ? (size_t)slots * p.npass * p.heads * D * D * sizeof(float) : 0;
+  return p.join != kWhole ? (size_t)slots * state_passes(p) * p.heads * D * D * sizeof(float) : 0;
 }
 
 template <class T, int D>
 hipError_t launch_passes(LinParams& p, int64_t slots, hipStream_t st) {
   const dim3 grid((unsigned)(slots * p.heads), p.npass), block(LinShape<D>::THREADS);
   if (p.join != kWhole)
-    hipLaunchKernelGGL((linear_kernel<T, D, true>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((linear_kernel<T, D, true>), dim3(grid.x, state_passes(p)), block, 0, st, p);
   if (p.join == kScanned)
     hipLaunchKernelGGL((linear_scan_kernel<D>),
-                       dim3((unsigned)(D * D / 1024 * p.batch * p.heads), p.npass), dim3(256), 0,
-                       st, p);
+                       dim3((unsigned)(D * D / 1024 * p.batch * p.heads), state_passes(p)),
+                       dim3(256), 0, st, p);
   hipLaunchKernelGGL((linear_kernel<T, D, false>), grid, block, 0, st, p);
   return hipGetLastError();
 }
@@ -956,16 +984,16 @@ LinParams bwd_params(const fa_linear_bwd_args& a) {
   pass(p.pass[0], o, v, k, a.dq, a.dq_stride, a.initial_state, a.is_stride, true);
   p.pass[0].p_scale = p.pass[0].inter_scale = a.scale;
   p.pass[0].upd_scale = 1.f;
-  pass(p.pass[1], v, o, q, a.dk, a.dk_stride, a.d_final_state, a.fs_stride, true);
-  pass(p.pass[2], k, q, o, a.dv, a.dv_stride, a.d_final_state, a.fs_stride, false);
+  pass(p.pass[1], k, q, o, a.dv, a.dv_stride, a.d_final_state, a.fs_stride, false);
+  pass(p.pass[kTwin], v, o, q, a.dk, a.dk_stride, a.d_final_state, a.fs_stride, true);
   for (int i = 1; i < 3; ++i) {
     // The carried state holds the scale (the final state's gradient has none).
     p.pass[i].reverse = 1;
     p.pass[i].p_scale = p.pass[i].upd_scale = a.scale;
     p.pass[i].inter_scale = 1.f;
   }
-  p.pass[2].fin = a.d_initial_state;
-  for (int i = 0; i < 2; ++i) p.pass[2].fs[i] = a.dis_stride[i];
+  p.pass[1].fin = a.d_initial_state;
+  for (int i = 0; i < 2; ++i) p.pass[1].fs[i] = a.dis_stride[i];
   p.log_decay = a.log_decay;
   p.batch = p.nstates = a.batch;
   p.seqlen = a.seqlen;
@@ -1050,7 +1078,7 @@ hipError_t launch_linear_bwd(const fa_linear_bwd_args& a, void* ws, hipStream_t 
   float* dv = dk + part / sizeof(float);
   if (part) {
     for (int i = 1; i < 3; ++i) {
-      p.pass[i].out = i == 1 ? dk : dv;
+      p.pass[i].out = i == kTwin ? dk : dv;
       p.pass[i].out_f32 = 1;
       p.pass[i].os[2] = a.head_dim;
       p.pass[i].os[1] = (int64_t)a.num_heads * a.head_dim;
