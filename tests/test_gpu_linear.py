@@ -454,3 +454,33 @@ def test_many_segments(case):
 @pytest.mark.parametrize("D", [64, 128])
 def test_many_packed_segments(lens, D):
     test_prefill_matches_reference(lens, 2, 1, D, torch.bfloat16)
+
+
+@pytest.mark.parametrize("D,H,S", [(64, 48, 8192), (128, 40, 5003), (256, 24, 3000)])
+def test_pool_is_read_before_it_is_written(D, H, S):
+    """Segments far beyond what the GPU runs at once, all starting from the state that
+    the last one replaces: the same as with two tensors, several times over."""
+    gen = torch.Generator().manual_seed(D)
+    q, k, v = (randn(gen, 1, S, H, D, dtype=torch.bfloat16).to(DEV) for _ in range(3))
+    g = slopes(H).to(DEV) / 64
+    first = (32 * torch.randn(1, H, D, D, generator=gen)).to(DEV)
+    want, final = fa.linear_attn_func(q, k, v, g, initial_state=first, return_final_state=True)
+    starts, prefix = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, S], [9]))
+    for _ in range(4):
+        pool = first.clone()
+        out = fa.linear_attn_prefill(q[0], k[0], v[0], g, pool, starts, prefix)
+        assert torch.equal(out, want[0]) and torch.equal(pool, final)
+
+
+def test_overlapping_offsets_stay_in_bounds():
+    """Sequences that claim the same rows have more segments than the workspace has
+    slots: no result is promised, the rows and slots of others are left alone."""
+    D, H, T = 64, 1, 4096
+    gen = torch.Generator().manual_seed(5)
+    q, k, v = (randn(gen, T, H, D, dtype=torch.float16).to(DEV) for _ in range(3))
+    starts = torch.tensor([0, T, 0, T, 0, T], dtype=torch.int32, device=DEV)
+    pool = torch.zeros(8, H, D, D, device=DEV)
+    fa.linear_attn_prefill(q, k, v, slopes(H).to(DEV), pool, starts,
+                           torch.ones(5, dtype=torch.int32, device=DEV))
+    torch.cuda.synchronize()
+    assert (pool[5:] == 0).all()

@@ -90,8 +90,10 @@ struct LinParams {
 };
 
 // How a segment comes by the state before it: there is one segment; from the
-// states of those before it, which the main kernel adds up; or linear_scan_kernel
-// has put it into its slot.
+// initial state and the states of those before it, which the main kernel adds up; or
+// linear_scan_kernel has put it into its slot.  (The main launch writes final states
+// where a pool's initial ones stand: with several segments it reads the copies that the
+// states' launch left in the last segments' slots.)
 enum { kWhole = 0, kAdded = 1, kScanned = 2 };
 // Passes: the forward alone, or dq, dv and dk, whose states are dv's transposed.
 constexpr int kTwin = 2;
@@ -371,7 +373,8 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
   const LinPass& a = p.pass[blockIdx.y];
   const Segment sg = find_segment(p, slot);
   if (sg.b < 0) return;
-  if (STATE_ONLY && sg.seg == sg.nseg - 1) return;  // no segment starts from it
+  // (No segment starts from the last one's state.)
+  if (STATE_ONLY && sg.seg == sg.nseg - 1 && (p.join != kAdded || sg.nseg == 1)) return;
   const int row0 = sg.seg * p.seglen;
   const int nrows = min(p.seglen, sg.len - row0);
 
@@ -400,8 +403,6 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
     load_rows<D>(sk, kp + t * a.k.s[1], a.k.s[1], step, n, tid);
     load_rows<D>(sv, vp + t * a.v.s[1], a.v.s[1], step, n, tid);
   };
-  load_chunk(0, threadIdx.x);
-
   // State column 16 wave + lc, rows 16 dt + 4 lq + (0..3).
   f32x4 S[L::DT];
   const bool twin = blockIdx.y == kTwin;
@@ -409,31 +410,45 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
   float* seg_state =
       p.ws + ((min((int)blockIdx.y, kTwin - 1) * slots + slot) * p.heads + h) * D * D;
   const int col = 16 * wave + lc;
+  const float* init = init_of(p, a, sg.b, h);
+  auto load_init = [&]() {
+#pragma unroll
+    for (int dt = 0; dt < L::DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        S[dt][i] = init[(16 * dt + 4 * lq + i) * a.ird + col * a.icd];
+  };
+  if (STATE_ONLY && sg.seg == sg.nseg - 1) {
+    if (!init) return;
+    load_init();
+#pragma unroll
+    for (int dt = 0; dt < L::DT; ++dt)
+      *reinterpret_cast<f32x4*>(seg_state + state_image<D>(wave, dt, lane)) = S[dt];
+    return;
+  }
+  load_chunk(0, threadIdx.x);
+
 #pragma unroll
   for (int dt = 0; dt < L::DT; ++dt) S[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (!STATE_ONLY) {
+    const int64_t next = (int64_t)p.heads * D * D;
     if (p.join == kScanned) {
       load_state<D>(S, seg_state, wave, lane, twin);
+    } else if (!kKeep || sg.nseg == 1) {
+      if (init) load_init();
     } else {
-      if (const float* src = init_of(p, a, sg.b, h)) {
+      // The initial state and those of the segments before, in order.  (Offsets that
+      // overlap would give more segments than there are slots.)
+      const int last = min(slot + sg.nseg - 1 - sg.seg, (int)slots - 1);
+      if (init) load_state<D>(S, seg_state + (last - slot) * next, wave, lane, twin);
+      const float decay = expm1f(g * (float)p.seglen);
+      for (int s = sg.seg; s > 0; --s) {
+        f32x4 x[L::DT];
+        load_state<D>(x, seg_state - s * next, wave, lane, twin);
 #pragma unroll
         for (int dt = 0; dt < L::DT; ++dt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            S[dt][i] = src[(16 * dt + 4 * lq + i) * a.ird + col * a.icd];
-      }
-      // The states of the segments before, in order.
-      if constexpr (kKeep) {
-        const float decay = expm1f(g * (float)p.seglen);
-        const int64_t next = (int64_t)p.heads * D * D;
-        for (int s = sg.seg; s > 0; --s) {
-          f32x4 x[L::DT];
-          load_state<D>(x, seg_state - s * next, wave, lane, twin);
-#pragma unroll
-          for (int dt = 0; dt < L::DT; ++dt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) S[dt][i] = fmaf(S[dt][i], decay, S[dt][i]) + x[dt][i];
-        }
+          for (int i = 0; i < 4; ++i) S[dt][i] = fmaf(S[dt][i], decay, S[dt][i]) + x[dt][i];
       }
     }
   }
