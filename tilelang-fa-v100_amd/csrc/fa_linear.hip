@@ -28,9 +28,9 @@
 // What bounds it: the chunks of a workgroup follow each other, and a chunk's phases
 // (operand reads, products, the split, barriers) hardly overlap.  At head_dim 128 a
 // chunk takes 3.4 us with 64 workgroups and 4.7 with 256 (long sequences, 3.6 TB/s);
-// of its 8416 cycles LDS is busy 49%, the matrix cores 29%, and the waves wait 41%.
+// of its 8540 cycles LDS is busy 49%, the matrix cores 28%, and the waves wait 42%.
 // [4, 2048, 16, 128] bf16: forward 43 us after 23 us for the segments' states,
-// the three gradients 128 us.
+// the three gradients 131 us.
 //
 // Registers and LDS: the state's accumulators (row d in the registers, column e
 // in the lane) are, rounded, the A operand of O^T = S^T Q^T as they stand: S never
@@ -724,7 +724,7 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
 // Joins the segments' states in order: each slot's own state becomes the state
 // before it.  A thread holds four components, in the workspace's layout
 // (state_image): rows d .. d + 3 of column e.  Bound by the states' memory: 9 us for
-// eight packed prompts of 16 heads at head_dim 128.
+// eight packed prompts of 16 heads at head_dim 128 (before those were added up).
 template <int D>
 __global__ __launch_bounds__(256) void linear_scan_kernel(LinParams p) {
   constexpr int PARTS = D * D / 1024;
@@ -795,7 +795,7 @@ __global__ __launch_bounds__(256) void linear_group_sum_kernel(const float* part
 // Bound by that memory (8 D^2 bytes a sequence and head; D^2 * 5 flops).  A
 // workgroup takes COLS columns of one head's state: every load is issued before
 // the first use, and a column's sum over d stays inside the workgroup.  64 x 32 states
-// at head_dim 128: 57 us, 4.7 TB/s (a large copy: 5.2); 4 x 16: 4.6 us.
+// at head_dim 128: 56 us, 4.8 TB/s (a large copy: 5.2); 4 x 16: 4.6 us.
 template <class T, int D, int COLS>
 __global__ __launch_bounds__(256) void linear_decode_kernel(fa_linear_decode_args a) {
   constexpr int LANES = COLS / 4, ROWS = 256 / LANES, N = D / ROWS, SLICES = D / COLS;
