@@ -19,7 +19,7 @@
 // Work split: a workgroup holds one (sequence, head, segment)'s state in
 // registers and walks its chunks; each wave owns 16 of the state's columns (D / 16
 // waves).  On a CU: three workgroups at head_dim 64 (registers, 41 KB of LDS), one at
-// 128 (two LDS buffers, 122 KB) and one at 256 (16 waves of 128 registers).  Where
+// 128 (two to three LDS buffers, 150 KB) and one at 256 (16 waves of 128 registers).  Where
 // sequences x heads are too few for the GPU, sequences are cut into segments: one
 // launch forms every segment's own state, and the main launch starts each segment
 // from the states of those before it, which it adds up itself (few segments) or finds
@@ -27,10 +27,10 @@
 //
 // What bounds it: the chunks of a workgroup follow each other, and a chunk's phases
 // (operand reads, products, the split, barriers) hardly overlap.  At head_dim 128 a
-// chunk takes 3.4 us with 64 workgroups and 4.7 with 256 (long sequences, 3.6 TB/s);
-// of its 8540 cycles LDS is busy 49%, the matrix cores 28%, and the waves wait 42%.
+// chunk takes 4.0 us with 256 workgroups (16 chunks, 68 us, 4.1 TB/s); of its 8420
+// cycles LDS is busy 49%, the matrix cores 29%, and the waves wait 43%.
 // [4, 2048, 16, 128] bf16: forward 43 us after 23 us for the segments' states,
-// the three gradients 131 us.
+// the three gradients 128 us.
 //
 // Registers and LDS: the state's accumulators (row d in the registers, column e
 // in the lane) are, rounded, the A operand of O^T = S^T Q^T as they stand: S never
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
   using Scores = typename L::Scores;
   constexpr int NT = kTerms<T>;
   // Whether registers hold what a chunk does not change (head_dim 256 has 128 of them
-  // for a wave, and spills 23 to 39 as it is).
+  // for a wave, and spills 20 to 36 as it is).
   constexpr bool kKeep = D < 256;
   // Buffers of a chunk's rows: with two, the next chunk's rows go to LDS while this
   // one is worked on, and one barrier of three goes: [2, 8192, 16, 128] forward 119 ->
@@ -364,8 +364,14 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
   constexpr int NB = D == 128 ? 2 : 1;
   __shared__ __align__(16) char lds_q[STATE_ONLY ? 16 : NB * Tile::kBytes];
   __shared__ __align__(16) char lds_k[NB * Tile::kBytes];
-  __shared__ __align__(16) char lds_v[NB * Tile::kBytes];
-  __shared__ __align__(16) char lds_p[STATE_ONLY ? 16 : Scores::kBytes];
+  // With two, a chunk's P meets V while the next chunk is worked on, which leaves one
+  // barrier a chunk: P has two buffers, and V, whose places take O's rows, three.  [32,
+  // 2048, 16, 128] backward 865 -> 844 us.  (Half of the waves with the state's products
+  // first and the rows and P after them: 872 us, 252 registers.)
+  constexpr bool kLate = NB == 2 && !STATE_ONLY;
+  constexpr int VB = kLate ? 3 : NB;
+  __shared__ __align__(16) char lds_v[VB * Tile::kBytes];
+  __shared__ __align__(16) char lds_p[STATE_ONLY ? 16 : NB * Scores::kBytes];
   __shared__ __align__(16) float weight[NB * kChunk];  // of row j in the state's update
   __shared__ float powers[STATE_ONLY ? 1 : kChunk + 17];
 
@@ -473,8 +479,8 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
   // The two tiles above the diagonal that O's 32-key steps take in.
   if (!STATE_ONLY && threadIdx.x < 64) {
     const int t = threadIdx.x >> 5, r = (threadIdx.x & 31) >> 1;
-    for (int g = 0; g < 2; ++g)
-      st8(lds_p + Scores::at(32 * t + r) + group_at(4 * (2 * t + 1) + 2 * (threadIdx.x & 1) + g),
+    for (int g = 0; g < 2 * NB; ++g)
+      st8(lds_p + (g >> 1) * Scores::kBytes + Scores::at(32 * t + r) + group_at(4 * (2 * t + 1) + 2 * (threadIdx.x & 1) + (g & 1)),
           u32x2{0, 0});
   }
 
@@ -501,7 +507,7 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
 
   // The rows of O that chunk c left in V's place, 16 bytes x 2 a thread (at the
   // places where the thread puts its part of a later V).
-  auto write_rows = [&](int c, int buf, int tid) {
+  auto write_rows = [&](int c, int vbuf, int tid) {
     const int n = min(kChunk, nrows - c);
     const rsrc_t rs = make_rsrc(static_cast<uint16_t*>(a.out) + batch * a.os[0] +
                                     lowest(c, n) * a.os[1] + h * a.os[2],
@@ -509,28 +515,157 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
 #pragma unroll
     for (int u = 0; u < 2; ++u)
       __builtin_amdgcn_raw_buffer_store_b128(
-          ld16(lds_v + buf * Tile::kBytes + place_of<D>(tid) + u * Tile::at(L::RPT)), rs,
+          ld16(lds_v + vbuf * Tile::kBytes + place_of<D>(tid) + u * Tile::at(L::RPT)), rs,
           row_offset(L::RPT * u + tid / L::CPR, n, step, 2 * (uint32_t)a.os[1],
                      16 * (tid % L::CPR)),
           0, 0);
   };
-  // Chunk c's rows, which have been loaded, and its weights into a buffer.
-  auto stage = [&](int c, int buf, int tid) {
+  // Chunk c's rows, which have been loaded, and its weights into their buffers.
+  auto stage = [&](int c, int buf, int vbuf, int tid) {
     if (!STATE_ONLY) store_grouped<D>(sq, lds_q + buf * Tile::kBytes, tid);
     store_rows<D>(sk, lds_k + buf * Tile::kBytes, tid);
-    store_rows<D>(sv, lds_v + buf * Tile::kBytes, tid);
+    store_rows<D>(sv, lds_v + vbuf * Tile::kBytes, tid);
     // Rows at or behind n are zeros: their weight only has to be finite.
     const int n = min(kChunk, nrows - c);
     if (tid < kChunk)
       weight[buf * kChunk + tid] = a.upd_scale * fast_exp2(g2 * (float)max(n - 1 - tid + sh, 0));
   };
   const bool out16 = !STATE_ONLY && !a.out_f32;
+  u32x4 vt[kChunk / 32];  // the wave's columns of V, for O and for the update
+  f32x4 o[4];
+  auto read_values = [&](const char* v_rows) {
+#pragma unroll
+    for (int s = 0; s < kChunk / 32; ++s)
+      vt[s] = read_transposed<Tile>(v_rows + tr_at + 32 * wave, s);
+  };
+  auto scores = [&](const char* q_rows, const char* k_rows, char* p_rows) {
+    // P^T = K Q^T with the decay, rounded, as P's rows in LDS.
+#pragma unroll
+    for (int np = 0; np < NP; ++np) {
+      const int tile = wave + L::NW * np;
+      if (tile < 10) {
+        const int it = (tile >= 1) + (tile >= 3) + (tile >= 6), jt = tile - it * (it + 1) / 2;
+        const char* kq = k_rows + Tile::at(16 * jt + lc) + 8 * lq;
+        const char* qq = q_rows + op_at + it * Tile::at(16);
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < D / 32; ++kk) {
+          const u32x2 x = ld8(kq + 64 * kk), y = ld8(kq + 64 * kk + 32);
+          acc = T::mma16(u32x4{x[0], x[1], y[0], y[1]}, ld16(qq + 64 * kk), acc);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] *= kKeep ? pf[np][i] : p_factor(tile, i);
+        st8(p_rows + p_at + it * Scores::at(16) + group_at(4 * jt + lq),
+            u32x2{T::pack(acc[0], acc[1]), T::pack(acc[2], acc[3])});
+      }
+    }
+  };
+  auto from_state = [&](const char* q_rows) {
+    // O^T = S^T Q^T, then the rows' decay.  fp16: S meets Q scaled by a power of
+    // two (its largest value to 2^14), so that neither a long memory's sums nor
+    // small ones leave the type's range.
+    float up = inter_scale, down = 1.f;
+    if constexpr (T::kId == 0) {
+      float m = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < L::DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(S[dt][i]));
+      m = __builtin_bit_cast(float, wave_max_nonneg(__builtin_bit_cast(int, m)));
+      const int e = m > 0.f && m < __builtin_inff() ? min(max(exponent(m), -100), 100) : 14;
+      down = pow2(14 - e);
+      up *= pow2(e - 14) * pow2(-held);
+    }
+#pragma unroll
+    for (int it = 0; it < 4; ++it) o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < L::DT; dt += 2) {
+      u32x4 sf;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sf[i] = T::pack(S[dt + i / 2][2 * (i & 1)] * down, S[dt + i / 2][2 * (i & 1) + 1] * down);
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+        o[it] = T::mma16(sf, ld16(q_rows + op_at + it * Tile::at(16) + 32 * dt), o[it]);
+    }
+#pragma unroll
+    for (int it = 0; it < 4; ++it) o[it] *= up * (kKeep ? rowf[it] : row_factor(it));
+  };
+  // The rest of chunk c's O, and O on its way out.
+  auto finish = [&](int c, const char* p_rows, char* v_rows) {
+    const int n = min(kChunk, nrows - c);
+    // O^T += V^T P^T
+#pragma unroll
+    for (int s = 0; s < kChunk / 32; ++s)
+#pragma unroll
+      for (int it = 2 * s; it < 4; ++it)
+        o[it] = T::mma16(vt[s], ld16(p_rows + p_at + it * Scores::at(16) + 64 * s + 16 * lq), o[it]);
+    if (a.out_f32) {
+      const rsrc_t rs = make_rsrc(static_cast<float*>(a.out) + batch * a.os[0] +
+                                      lowest(c, n) * a.os[1] + h * a.os[2],
+                                  (uint32_t)((n - 1) * a.os[1] + D) * 4u);
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+        __builtin_amdgcn_raw_buffer_store_b128(
+            __builtin_bit_cast(u32x4, o[it]), rs,
+            row_offset(16 * it + lc, n, step, 4 * (uint32_t)a.os[1], 4 * (16 * wave + 4 * lq)), 0,
+            0);
+    } else {
+      // Into V's columns of this wave, which no other wave reads.
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+        st8(v_rows + Tile::at(16 * it + lc) + 32 * wave + 8 * lq,
+            u32x2{T::pack(o[it][0], o[it][1]), T::pack(o[it][2], o[it][3])});
+    }
+  };
+  auto update = [&](const char* k_rows, int buf) {
+    // S = l^n S + K^T (weight V).  The decay as S + S (l^n - 1): the factor's own
+    // rounding, which a slow decay would compound over hundreds of chunks, is then
+    // relative to the small difference.
+#pragma unroll
+    for (int dt = 0; dt < L::DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) S[dt][i] = fmaf(S[dt][i], dm1, S[dt][i]);
+    if constexpr (T::kId == 0) {
+      const int e = max_exponent(vt);
+      const int want = 13 - e - weight_top;
+      // Down where a term would overflow, up where eight bits would be lost.
+      if (e != kNone && (want < held || want > held + 8)) {
+        const float f = pow2(want - held);
+#pragma unroll
+        for (int dt = 0; dt < L::DT; ++dt) S[dt] *= f;
+        held = want;
+      }
+    }
+    const float hold = T::kId == 0 ? pow2(held) : 1.f;
+#pragma unroll
+    for (int s = 0; s < kChunk / 32; ++s) {
+      float x[8];
+      const float* w = weight + buf * kChunk + 32 * s + 4 * lq;
+      const f32x4 w0 = *reinterpret_cast<const f32x4*>(w) * hold;
+      const f32x4 w1 = *reinterpret_cast<const f32x4*>(w + 16) * hold;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = T::lo(vt[s][i]) * (i < 2 ? w0[2 * i] : w1[2 * i - 4]);
+        x[2 * i + 1] = T::hi(vt[s][i]) * (i < 2 ? w0[2 * i + 1] : w1[2 * i - 3]);
+      }
+      u32x4 term[NT];
+      split_terms<T, NT>(x, term);
+#pragma unroll
+      for (int dt = 0; dt < L::DT; ++dt) {
+        const u32x4 kt = read_transposed<Tile>(k_rows + tr_at + 32 * dt, s);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) S[dt] = T::mma16(kt, term[t], S[dt]);
+      }
+    }
+  };
+
   if constexpr (NB == 2) {
-    stage(0, 0, threadIdx.x);
+    stage(0, 0, 0, threadIdx.x);
     if (kChunk < nrows) load_chunk(kChunk, threadIdx.x);
     __syncthreads();
   }
-
+  int vbuf = 0;  // V's buffer of the chunk
   for (int c = 0; c < nrows; c += kChunk) {
     const int n = min(kChunk, nrows - c);
     const int buf = NB == 2 ? c / kChunk & 1 : 0;
@@ -539,165 +674,55 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
     // their way.
     int tid = threadIdx.x;
     if constexpr (!kKeep) asm volatile("" : "+v"(tid));
-    if constexpr (NB == 1) {
-      __syncthreads();  // the last chunk's LDS reads are done, and its O is there
-      if (out16 && c > 0) write_rows(c - kChunk, 0, tid);
-      stage(c, 0, tid);
-      __syncthreads();
-      if (c + kChunk < nrows) load_chunk(c + kChunk, tid);
-    }
-    // The next chunk into the other buffer, whose readers were done before the last
-    // barrier, and the last chunk's O out of it.
-    auto turn_over = [&]() {
-      if constexpr (NB == 2) {
-        if (out16 && c > 0) write_rows(c - kChunk, buf ^ 1, tid);
-        if (c + kChunk < nrows) stage(c + kChunk, buf ^ 1, tid);
-        if (c + 2 * kChunk < nrows) load_chunk(c + 2 * kChunk, tid);
-      }
-    };
     if (c == 0 || n < kChunk) dm1 = expm1f(g * (float)n);
     const char* q_rows = lds_q + buf * Tile::kBytes;
     const char* k_rows = lds_k + buf * Tile::kBytes;
-    char* v_rows = lds_v + buf * Tile::kBytes;
-
-    u32x4 vt[kChunk / 32];  // the wave's columns of V, for O and for the update
-#pragma unroll
-    for (int s = 0; s < kChunk / 32; ++s) vt[s] = read_transposed<Tile>(v_rows + tr_at + 32 * wave, s);
-    f32x4 o[4];
-    if constexpr (!STATE_ONLY) {
-      // P^T = K Q^T with the decay, rounded, as P's rows in LDS.
-#pragma unroll
-      for (int np = 0; np < NP; ++np) {
-        const int tile = wave + L::NW * np;
-        if (tile < 10) {
-          const int it = (tile >= 1) + (tile >= 3) + (tile >= 6), jt = tile - it * (it + 1) / 2;
-          const char* kq = k_rows + Tile::at(16 * jt + lc) + 8 * lq;
-          const char* qq = q_rows + op_at + it * Tile::at(16);
-          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int kk = 0; kk < D / 32; ++kk) {
-            const u32x2 x = ld8(kq + 64 * kk), y = ld8(kq + 64 * kk + 32);
-            acc = T::mma16(u32x4{x[0], x[1], y[0], y[1]}, ld16(qq + 64 * kk), acc);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] *= kKeep ? pf[np][i] : p_factor(tile, i);
-          st8(lds_p + p_at + it * Scores::at(16) + group_at(4 * jt + lq),
-              u32x2{T::pack(acc[0], acc[1]), T::pack(acc[2], acc[3])});
-        }
-      }
-      // O^T = S^T Q^T, then the rows' decay.  fp16: S meets Q scaled by a power of
-      // two (its largest value to 2^14), so that neither a long memory's sums nor
-      // small ones leave the type's range.
-      float up = inter_scale, down = 1.f;
-      if constexpr (T::kId == 0) {
-        float m = 0.f;
-#pragma unroll
-        for (int dt = 0; dt < L::DT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(S[dt][i]));
-        m = __builtin_bit_cast(float, wave_max_nonneg(__builtin_bit_cast(int, m)));
-        const int e = m > 0.f && m < __builtin_inff() ? min(max(exponent(m), -100), 100) : 14;
-        down = pow2(14 - e);
-        up *= pow2(e - 14) * pow2(-held);
-      }
-#pragma unroll
-      for (int it = 0; it < 4; ++it) o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int dt = 0; dt < L::DT; dt += 2) {
-        u32x4 sf;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          sf[i] = T::pack(S[dt + i / 2][2 * (i & 1)] * down, S[dt + i / 2][2 * (i & 1) + 1] * down);
-#pragma unroll
-        for (int it = 0; it < 4; ++it)
-          o[it] = T::mma16(sf, ld16(q_rows + op_at + it * Tile::at(16) + 32 * dt), o[it]);
-      }
-#pragma unroll
-      for (int it = 0; it < 4; ++it) o[it] *= up * (kKeep ? rowf[it] : row_factor(it));
-    }
-
-    auto finish = [&]() {
-      __syncthreads();  // P is there
-      turn_over();
-      // O^T += V^T P^T
-#pragma unroll
-      for (int s = 0; s < kChunk / 32; ++s)
-#pragma unroll
-        for (int it = 2 * s; it < 4; ++it)
-          o[it] = T::mma16(vt[s], ld16(lds_p + p_at + it * Scores::at(16) + 64 * s + 16 * lq), o[it]);
-      if (a.out_f32) {
-        const rsrc_t rs = make_rsrc(static_cast<float*>(a.out) + batch * a.os[0] +
-                                        lowest(c, n) * a.os[1] + h * a.os[2],
-                                    (uint32_t)((n - 1) * a.os[1] + D) * 4u);
-#pragma unroll
-        for (int it = 0; it < 4; ++it)
-          __builtin_amdgcn_raw_buffer_store_b128(
-              __builtin_bit_cast(u32x4, o[it]), rs,
-              row_offset(16 * it + lc, n, step, 4 * (uint32_t)a.os[1], 4 * (16 * wave + 4 * lq)), 0,
-              0);
+    char* p_rows = lds_p + (STATE_ONLY ? 0 : buf * Scores::kBytes);
+    if constexpr (kLate) {
+      const int next = vbuf == 2 ? 0 : vbuf + 1, before = vbuf == 0 ? 2 : vbuf - 1;
+      if (c > 0)
+        finish(c - kChunk, lds_p + (buf ^ 1) * Scores::kBytes, lds_v + before * Tile::kBytes);
+      // The next chunk's rows, into buffers whose readers were done before the last
+      // barrier; in V's stands the O of two chunks ago.
+      if (out16 && c > kChunk) write_rows(c - 2 * kChunk, next, tid);
+      if (c + kChunk < nrows) stage(c + kChunk, buf ^ 1, next, tid);
+      if (c + 2 * kChunk < nrows) load_chunk(c + 2 * kChunk, tid);
+      read_values(lds_v + vbuf * Tile::kBytes);
+      scores(q_rows, k_rows, p_rows);
+      from_state(q_rows);
+      update(k_rows, buf);
+      vbuf = next;
+      __syncthreads();  // P and the next chunk are there, and O of the chunk before
+    } else if constexpr (STATE_ONLY) {
+      if constexpr (NB == 2) {
+        if (c + kChunk < nrows) stage(c + kChunk, buf ^ 1, buf ^ 1, tid);
+        if (c + 2 * kChunk < nrows) load_chunk(c + 2 * kChunk, tid);
       } else {
-        // Into V's columns of this wave, which no other wave reads.
-#pragma unroll
-        for (int it = 0; it < 4; ++it)
-          st8(v_rows + Tile::at(16 * it + lc) + 32 * wave + 8 * lq,
-              u32x2{T::pack(o[it][0], o[it][1]), T::pack(o[it][2], o[it][3])});
+        __syncthreads();  // the last chunk's LDS reads are done
+        stage(c, 0, 0, tid);
+        __syncthreads();
+        if (c + kChunk < nrows) load_chunk(c + kChunk, tid);
       }
-    };
-    auto update = [&]() {
-      // S = l^n S + K^T (weight V).  The decay as S + S (l^n - 1): the factor's own
-      // rounding, which a slow decay would compound over hundreds of chunks, is then
-      // relative to the small difference.
-#pragma unroll
-      for (int dt = 0; dt < L::DT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) S[dt][i] = fmaf(S[dt][i], dm1, S[dt][i]);
-      if constexpr (T::kId == 0) {
-        const int e = max_exponent(vt);
-        const int want = 13 - e - weight_top;
-        // Down where a term would overflow, up where eight bits would be lost.
-        if (e != kNone && (want < held || want > held + 8)) {
-          const float f = pow2(want - held);
-#pragma unroll
-          for (int dt = 0; dt < L::DT; ++dt) S[dt] *= f;
-          held = want;
-        }
-      }
-      const float hold = T::kId == 0 ? pow2(held) : 1.f;
-#pragma unroll
-      for (int s = 0; s < kChunk / 32; ++s) {
-        float x[8];
-        const float* w = weight + buf * kChunk + 32 * s + 4 * lq;
-        const f32x4 w0 = *reinterpret_cast<const f32x4*>(w) * hold;
-        const f32x4 w1 = *reinterpret_cast<const f32x4*>(w + 16) * hold;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[2 * i] = T::lo(vt[s][i]) * (i < 2 ? w0[2 * i] : w1[2 * i - 4]);
-          x[2 * i + 1] = T::hi(vt[s][i]) * (i < 2 ? w0[2 * i + 1] : w1[2 * i - 3]);
-        }
-        u32x4 term[NT];
-        split_terms<T, NT>(x, term);
-#pragma unroll
-        for (int dt = 0; dt < L::DT; ++dt) {
-          const u32x4 kt = read_transposed<Tile>(k_rows + tr_at + 32 * dt, s);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) S[dt] = T::mma16(kt, term[t], S[dt]);
-        }
-      }
-    };
-    // The update stands before the barrier that P's readers need, where the waves
-    // that formed P's tiles are behind the others; at head_dim 256 there are no
-    // registers to keep O through it.
-    if constexpr (STATE_ONLY) {
-      turn_over();
-      update();
-    } else if constexpr (D < 256) {
-      update();
-      finish();
+      read_values(lds_v + buf * Tile::kBytes);
+      update(k_rows, buf);
+      if constexpr (NB == 2) __syncthreads();  // the next chunk is there
     } else {
-      finish();
-      update();
+      __syncthreads();  // the last chunk's LDS reads are done, and its O is there
+      if (out16 && c > 0) write_rows(c - kChunk, 0, tid);
+      stage(c, 0, 0, tid);
+      __syncthreads();
+      if (c + kChunk < nrows) load_chunk(c + kChunk, tid);
+      read_values(lds_v);
+      scores(q_rows, k_rows, p_rows);
+      from_state(q_rows);
+      // The update stands before the barrier that P's readers need, where the waves
+      // that formed P's tiles are behind the others; at head_dim 256 there are no
+      // registers to keep O through it.
+      if constexpr (kKeep) update(k_rows, 0);
+      __syncthreads();  // P is there
+      finish(c, p_rows, lds_v);
+      if constexpr (!kKeep) update(k_rows, 0);
     }
-    if constexpr (NB == 2) __syncthreads();  // the next chunk is there, and this one's O
   }
 
   const float out = pow2(-held);
@@ -707,10 +732,15 @@ __global__ __launch_bounds__(LinShape<D>::THREADS, D == 256 ? 4 : 2) void linear
       *reinterpret_cast<f32x4*>(seg_state + state_image<D>(wave, dt, lane)) = S[dt] * out;
     return;
   }
+  const int c = (nrows - 1) / kChunk * kChunk;
+  if constexpr (kLate) {
+    vbuf = vbuf == 0 ? 2 : vbuf - 1;
+    finish(c, lds_p + (c / kChunk & 1) * Scores::kBytes, lds_v + vbuf * Tile::kBytes);
+    if (out16 && c > 0) write_rows(c - kChunk, vbuf == 0 ? 2 : vbuf - 1, threadIdx.x);
+  }
   if (out16) {
     __syncthreads();
-    const int c = (nrows - 1) / kChunk * kChunk;
-    write_rows(c, NB == 2 ? c / kChunk & 1 : 0, threadIdx.x);
+    write_rows(c, vbuf, threadIdx.x);
   }
   float* fin = sg.seg == sg.nseg - 1 ? fin_of(p, a, sg.b, h) : nullptr;
   if (fin) {
