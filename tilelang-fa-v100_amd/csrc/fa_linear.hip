@@ -900,7 +900,7 @@ double launch_us(int64_t groups, int64_t chunks, int per_cu, double lat, double 
 // twice and carried through memory: the count with the least time by the model
 // above.  Its constants (us a chunk, TB/s) are fitted to MI355X times of the forward
 // and the backward of 21 shapes, one to forty heads and 1024 to 32768 rows, at 1 to 64
-// segments: what it picks is within 3% of the fastest of them, 0.3% on average.
+// segments: what it picks is within 4% of the fastest of them, 0.3% on average.
 // units: sequences x heads x passes; state_units: of those, the ones whose segments'
 // states are formed.  tokens: of one sequence, or of all `seqs` packed ones, which end
 // in a part of a segment each.
